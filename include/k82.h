@@ -179,6 +179,126 @@ int k82_pcm16(k82_handle* h, const float* src, int16_t* dst, int64_t n, void* st
 #define K82_PCM16_STATIC_MAX (4 * 1024 * 1024)
 int k82_pcm16_static(k82_handle* h, const float* src, int16_t* dst, int64_t n, void* stream);
 
+/* ---- operators on the caller's own device tensors --------------------------------------
+ *
+ * Per-request weights beside the model's shared ones: low-rank adapters of many requests at once next to a shared
+ * projection, and layer norm with a gain and an offset per request; both forward and backward, so that adapters can be
+ * trained and served with the same numbers.  The reference has no counterpart (its voices are style vectors only).
+ *
+ * Any handle will do, also one without weights (k82_create alone).  All tensors are device memory of the handle's GPU.
+ * `stream` NULL: the handle's own stream, and the call returns when the result is there, like every other entry point.
+ * Any other stream (hipStreamLegacy for the default stream): the call only enqueues, synchronises nothing, allocates
+ * nothing and may be captured into a graph; segments are host arrays, read before the call returns.
+ *
+ * Layout of a tensor [tokens][channels]: K82_ROWS element (t, c) at p[t * ld + c], ld >= channels; K82_COLS, the
+ * engine's own channel-first layout, at p[c * ld + t], ld >= tokens.  K82_COLS exists in K82_F32 only and in the forward
+ * operators only.  All tensors of a call share dtype and layout unless stated; no alignment beyond the element's own is
+ * needed.
+ *
+ * Segments cut the token axis: segment s holds the tokens [off[s], off[s+1]), 0 <= off[0] <= ... <= off[n] <= tokens,
+ * and uses adapter (gain) index[s]; an index may come any number of times and a segment may be empty.  Output rows that
+ * no segment holds are left as they were. */
+#define K82_F32 0
+#define K82_BF16 1
+#define K82_ROWS 0
+#define K82_COLS 1
+#define K82_ACT_NONE 0
+#define K82_ACT_GELU_NEW 1
+#define K82_LORA_MAX_RANK 128
+
+typedef struct k82_segments {
+    const int64_t* off;   /* host i64[n + 1] */
+    const int32_t* index; /* host i32[n] */
+    int32_t n;            /* >= 0 */
+} k82_segments;
+
+/* y = act(base + scale[k] * (x A_k^T) B_k^T), k = index of the token's segment; k = -1: y = act(base).
+ * base is what the shared projection wrote (NULL: 0) and may be y itself; x and y must not overlap.  Products of 16-bit
+ * operands are exact, all sums are 32 bits wide, and y is rounded once.
+ * h (NULL: not kept): f32[tokens][rank], x A_k^T (0 where k = -1), which k82_op_lora_grad takes. */
+typedef struct k82_lora {
+    int32_t dtype, layout, act;
+    int32_t cin, cout, rank, adapters;
+    int64_t tokens;
+    const void* x; int64_t ldx;
+    const void* base; int64_t ldbase;
+    void* y; int64_t ldy;
+    const void* a;        /* [adapters][rank][cin], dtype */
+    const void* b;        /* [adapters][cout][rank], dtype */
+    const float* scale;   /* device f32[adapters] */
+    float* h;
+} k82_lora;
+int k82_op_lora(k82_handle* h, const k82_lora* p, const k82_segments* seg, void* stream);
+
+/* Backward of k82_op_lora without activation (dy: the gradient in front of act), K82_ROWS:
+ *   dx = dx_base + scale[k] (dy B_k) A_k   (k = -1: dx = dx_base; dx_base NULL: 0; dx_base may be dx itself)
+ *   da_k = scale[k] sum_t (dy B_k)^T x,  db_k = scale[k] sum_t dy^T h   (f32; zero for an adapter without tokens)
+ * Sums over tokens are taken in a fixed order: the same call gives the same bits.  dx may not overlap x or dy.
+ * workspace: device memory of at least k82_op_lora_grad_workspace bytes, 256-byte aligned, the caller's until the
+ * enqueued work is done. */
+typedef struct k82_lora_grad {
+    int32_t dtype;
+    int32_t cin, cout, rank, adapters;
+    int64_t tokens;
+    const void* x; int64_t ldx;
+    const void* dy; int64_t lddy;
+    const float* h;       /* f32[tokens][rank], as k82_op_lora kept it */
+    const void* dx_base; int64_t lddx_base;
+    void* dx; int64_t lddx;
+    const void* a;
+    const void* b;
+    const float* scale;
+    float* da;            /* f32[adapters][rank][cin] */
+    float* db;            /* f32[adapters][cout][rank] */
+} k82_lora_grad;
+int k82_op_lora_grad(k82_handle* h, const k82_lora_grad* p, const k82_segments* seg, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+/* Bytes of workspace, or K82_EINVAL for arguments that k82_op_lora_grad refuses (needs no GPU; reason:
+ * k82_last_error(NULL)). */
+int64_t k82_op_lora_grad_workspace(const k82_lora_grad* p, const k82_segments* seg);
+
+/* z = x + res (res NULL: z = x); y = (z - mean) * rstd * gain_k + offset_k over the channels of a token,
+ * rstd = 1 / sqrt(var + eps), var the mean square around the mean.  0 <= k < gains.  y may be x or res itself.
+ * mean, rstd (both or neither): f32[tokens], which k82_op_layernorm_grad takes. */
+typedef struct k82_layernorm {
+    int32_t dtype, layout;
+    int32_t c, gains;
+    float eps;
+    int64_t tokens;
+    const void* x; int64_t ldx;
+    const void* res; int64_t ldres;
+    void* y; int64_t ldy;
+    const void* gain;     /* [gains][c], dtype */
+    const void* offset;   /* [gains][c], dtype */
+    float* mean;
+    float* rstd;
+} k82_layernorm;
+int k82_op_layernorm(k82_handle* h, const k82_layernorm* p, const k82_segments* seg, void* stream);
+
+/* Backward of k82_op_layernorm, K82_ROWS: with xh = (x + res - mean) * rstd and u = dy * gain_k,
+ *   dx = rstd * (u - mean_c(u) - xh * mean_c(u xh))   (the gradient of x and of res alike; may be dy, x or res itself)
+ *   dgain_k = sum_t dy xh,  doffset_k = sum_t dy      (f32; zero for a gain without tokens; fixed order) */
+typedef struct k82_layernorm_grad {
+    int32_t dtype;
+    int32_t c, gains;
+    int64_t tokens;
+    const void* x; int64_t ldx;
+    const void* res; int64_t ldres;
+    const void* dy; int64_t lddy;
+    void* dx; int64_t lddx;
+    const void* gain;
+    const float* mean;
+    const float* rstd;
+    float* dgain;         /* f32[gains][c] */
+    float* doffset;       /* f32[gains][c] */
+} k82_layernorm_grad;
+int k82_op_layernorm_grad(k82_handle* h, const k82_layernorm_grad* p, const k82_segments* seg, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+int64_t k82_op_layernorm_grad_workspace(const k82_layernorm_grad* p, const k82_segments* seg);
+/* The same checks for the forward operators, without a GPU: K82_OK or K82_EINVAL with k82_last_error(NULL). */
+int k82_op_lora_check(const k82_lora* p, const k82_segments* seg);
+int k82_op_layernorm_check(const k82_layernorm* p, const k82_segments* seg);
+
 /* ---- measurement and test hooks (no counterpart in the reference) ---------------------- */
 
 /* Per-kernel-family timing with HIP events on the engine's stream (bench.py roofline leg).

@@ -1,0 +1,187 @@
+"""Refusals of the operators on caller-owned tensors (include/k82.h): the library's own checks need no GPU, and the Python
+face refuses before it reaches the library."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from tts_amd import Operators, Segments, _lib
+
+P = 1 << 20                      # pointers that nothing reads
+
+
+def lora(**kw):
+    d = dict(dtype=0, layout=0, act=0, cin=16, cout=24, rank=4, adapters=2, tokens=10, x=P, ldx=16, base=None, ldbase=0,
+             y=2 * P, ldy=24, a=3 * P, b=4 * P, scale=5 * P, h=None)
+    return _lib.K82Lora(**{**d, **kw})
+
+
+def lora_grad(**kw):
+    d = dict(dtype=0, cin=16, cout=24, rank=4, adapters=2, tokens=10, x=P, ldx=16, dy=2 * P, lddy=24, h=3 * P, dx_base=None,
+             lddx_base=0, dx=4 * P, lddx=16, a=5 * P, b=6 * P, scale=7 * P, da=8 * P, db=9 * P)
+    return _lib.K82LoraGrad(**{**d, **kw})
+
+
+def norm(**kw):
+    d = dict(dtype=0, layout=0, c=16, gains=2, eps=1e-5, tokens=10, x=P, ldx=16, res=None, ldres=0, y=2 * P, ldy=16,
+             gain=3 * P, offset=4 * P, mean=None, rstd=None)
+    return _lib.K82Layernorm(**{**d, **kw})
+
+
+def norm_grad(**kw):
+    d = dict(dtype=0, c=16, gains=2, tokens=10, x=P, ldx=16, res=None, ldres=0, dy=2 * P, lddy=16, dx=3 * P, lddx=16,
+             gain=4 * P, mean=5 * P, rstd=6 * P, dgain=7 * P, doffset=8 * P)
+    return _lib.K82LayernormGrad(**{**d, **kw})
+
+
+def raw_segments(off, index):
+    """A k82_segments of unchecked values (the arrays stay alive through the returned object)."""
+    o, i = np.array(off, np.int64), np.array(index, np.int32)
+    s = _lib.K82Segments(off=o.ctypes.data, index=i.ctypes.data, n=i.size)
+    s.keep = (o, i)
+    return s
+
+
+FUNCTIONS = {"lora": (lora, "k82_op_lora_check"), "lora_grad": (lora_grad, "k82_op_lora_grad_workspace"),
+             "norm": (norm, "k82_op_layernorm_check"), "norm_grad": (norm_grad, "k82_op_layernorm_grad_workspace")}
+
+
+def answer(which, seg=None, **kw):
+    lib = _lib.load()
+    make, name = FUNCTIONS[which]
+    rc = getattr(lib, name)(make(**kw), seg if seg is not None else raw_segments([0, 4, 10], [0, 1]))
+    return rc, lib.k82_last_error(None).decode() if rc < 0 else ""
+
+
+@pytest.mark.parametrize("which", FUNCTIONS)
+def test_ordinary_arguments_are_accepted(which):
+    for kw in ({}, {"tokens": 0, "x": None}, {"dtype": 1}):
+        seg = raw_segments([0], []) if kw.get("tokens") == 0 else None
+        assert answer(which, seg, **kw)[0] >= 0, kw
+    # empty segments, an index that comes twice, rows that no segment holds
+    assert answer(which, raw_segments([2, 2, 5, 5, 9], [0, 1, 1, 0]))[0] >= 0
+
+
+@pytest.mark.parametrize("which,kw,word", [
+    ("lora", dict(dtype=2), "dtype"), ("lora", dict(layout=2), "layout"), ("lora", dict(layout=1, dtype=1), "K82_F32 only"),
+    ("lora", dict(act=7), "act"), ("lora", dict(rank=0), "rank"), ("lora", dict(rank=129), "rank"),
+    ("lora", dict(cin=0), "channel"), ("lora", dict(cout=-1), "channel"), ("lora", dict(tokens=-1), "tokens"),
+    ("lora", dict(tokens=1 << 31), "tokens"), ("lora", dict(x=None), "x must not"), ("lora", dict(y=None), "y must not"),
+    ("lora", dict(a=None), "a, b and scale"), ("lora", dict(scale=None), "a, b and scale"),
+    ("lora", dict(adapters=-1), "adapters"), ("lora", dict(ldx=15), "ld of x"), ("lora", dict(ldy=0), "ld of y"),
+    ("lora", dict(base=6 * P, ldbase=23), "ld of base"), ("lora", dict(x=P + 2), "aligned"),
+    ("lora", dict(y=P), "overlap"), ("lora", dict(y=P + 8 * 4), "overlap"), ("lora", dict(base=2 * P + 4, ldbase=24), "overlap"),
+    ("lora", dict(base=2 * P, ldbase=25, ldy=24), "overlap"), ("lora", dict(h=2 * P), "overlaps"),
+    ("lora", dict(layout=1, ldx=9, ldy=10), "ld of x"),
+    ("lora_grad", dict(dtype=3), "dtype"), ("lora_grad", dict(rank=200), "rank"), ("lora_grad", dict(h=None), "h must not"),
+    ("lora_grad", dict(da=None), "da and db"), ("lora_grad", dict(dx=P), "overlaps"), ("lora_grad", dict(dx=2 * P), "overlaps"),
+    ("lora_grad", dict(dx_base=4 * P + 4, lddx_base=16), "without being one"), ("lora_grad", dict(lddy=23), "ld of dy"),
+    ("norm", dict(c=0), "channel"), ("norm", dict(gains=0), "gain"), ("norm", dict(gain=None), "gain"),
+    ("norm", dict(eps=-1.0), "eps"), ("norm", dict(eps=float("nan")), "eps"), ("norm", dict(mean=6 * P), "come together"),
+    ("norm", dict(layout=1, dtype=1), "K82_F32 only"), ("norm", dict(y=P + 4), "overlap"), ("norm", dict(ldx=15), "ld of x"),
+    ("norm", dict(mean=2 * P, rstd=9 * P), "overlaps"),
+    ("norm_grad", dict(mean=None), "mean and rstd"), ("norm_grad", dict(dgain=None), "dgain"),
+    ("norm_grad", dict(dx=P + 4), "overlaps"), ("norm_grad", dict(dx=5 * P), "overlaps mean"), ("norm_grad", dict(dy=None), "dy must not"),
+])
+def test_bad_arguments_are_refused(which, kw, word):
+    rc, msg = answer(which, **kw)
+    assert rc == -22 and word in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("which", FUNCTIONS)
+@pytest.mark.parametrize("off,index,word", [
+    ([0, 5, 4], [0, 1], "decrease"), ([-1, 4, 10], [0, 1], "negative"), ([0, 4, 11], [0, 1], "10 tokens"),
+    ([0, 4, 10], [0, 2], "index 2"), ([0, 4, 10], [-2, 1], "index -2"),
+])
+def test_bad_segments_are_refused(which, off, index, word):
+    rc, msg = answer(which, raw_segments(off, index))
+    assert rc == -22 and word in msg, (rc, msg)
+
+
+def test_no_adapter_is_for_adapters_only():
+    for which in ("lora", "lora_grad"):
+        assert answer(which, raw_segments([0, 10], [-1]))[0] >= 0
+        assert answer(which, raw_segments([0, 10], [-1]), adapters=0, a=None, b=None, scale=None)[0] >= 0
+    for which in ("norm", "norm_grad"):
+        assert answer(which, raw_segments([0, 10], [-1]))[0] == -22
+
+
+def test_shared_buffers_that_do_not_overlap_are_accepted():
+    # x and y are column ranges of one buffer; base is y; dx is dx_base; the norm works in place
+    assert answer("lora", x=P, ldx=40, y=P + 16 * 4, ldy=40)[0] == 0
+    assert answer("lora", x=P, ldx=40, y=P + 15 * 4, ldy=40)[0] == -22
+    assert answer("lora", base=2 * P, ldbase=24)[0] == 0
+    assert answer("lora", layout=1, x=P, ldx=32, y=P + 16 * 32 * 4, ldy=32)[0] == 0
+    assert answer("lora_grad", dx_base=4 * P, lddx_base=16)[0] >= 0
+    assert answer("norm", y=P, ldy=16)[0] == 0
+    for d in (P, 2 * P):
+        assert answer("norm_grad", dx=d)[0] >= 0
+
+
+def test_null_arguments_are_refused():
+    lib = _lib.load()
+    seg = raw_segments([0, 10], [0])
+    assert lib.k82_op_lora_check(None, seg) == -22 and lib.k82_op_layernorm_check(None, seg) == -22
+    assert lib.k82_op_lora_grad_workspace(None, seg) == -22 and lib.k82_op_layernorm_grad_workspace(None, seg) == -22
+    assert lib.k82_op_lora_check(lora(), None) == -22
+    bad = _lib.K82Segments(off=None, index=None, n=2)
+    assert lib.k82_op_lora_check(lora(), bad) == -22
+    assert lib.k82_op_lora_check(lora(), _lib.K82Segments(off=None, index=None, n=-1)) == -22
+    assert lib.k82_op_lora(None, lora(), seg, None) == -22        # no handle
+
+
+def test_segments_class_refuses_what_is_not_a_cut():
+    s = Segments.of_lengths([3, 0, 4], [1, 0, -1])
+    assert s.offsets.tolist() == [0, 3, 3, 7] and (s.lo, s.hi) == (0, 7)
+    for off, index in (([0, 2], [0, 1]), ([0, 3, 2], [0, 1]), ([-1, 3], [0]), ([[0, 1]], [0])):
+        with pytest.raises(ValueError):
+            Segments(off, index)
+    with pytest.raises(ValueError):
+        s.offsets[0] = 5                                        # the library reads this memory
+
+
+def test_python_face_refuses_before_the_library():
+    ops = object.__new__(Operators)                              # no GPU here: a face without a handle
+    ops.device, ops.h = 0, C.c_void_p()
+    x, a, b, s = torch.zeros(4, 8), torch.zeros(1, 2, 8), torch.zeros(1, 6, 2), torch.ones(1)
+    with pytest.raises(ValueError, match="must be on cuda:0"):
+        ops.op_lora(x, a, b, s)
+    with pytest.raises(TypeError, match="torch tensor"):
+        ops.op_lora(x.numpy(), a, b, s)
+    with pytest.raises(ValueError, match="must be on cuda:0"):
+        ops.op_layernorm(x, torch.ones(1, 8), torch.ones(1, 8))
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        ops._dtype(x.half())
+    with pytest.raises(TypeError, match="b is"):
+        ops._dtype(x, b=b.bfloat16())
+    with pytest.raises(ValueError, match="two dimensions"):
+        ops._layout(x=x[None])
+    with pytest.raises(ValueError, match="share one layout"):
+        ops._layout(x=x, base=torch.zeros(6, 4).t())             # rows beside channel-first
+    with pytest.raises(ValueError, match="share one layout"):
+        ops._layout(x=torch.zeros(1, 8).expand(4, 8))            # rows that lie on each other
+    with pytest.raises(ValueError, match="share one layout"):
+        ops._layout(True, x=torch.zeros(8, 4).t())               # the backward pass takes rows
+    with pytest.raises(ValueError, match="scale has shape"):
+        ops._factors(x, a, b, torch.ones(2))
+    with pytest.raises(ValueError, match="b has shape"):
+        ops._factors(x, a, torch.zeros(1, 6, 3), s)
+    with pytest.raises(ValueError, match="x has shape"):
+        ops._factors(torch.zeros(4, 7), a, b, s)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops._factors(x, torch.zeros(1, 8, 2).transpose(1, 2), b, s)
+    with pytest.raises(ValueError, match="end at token 5"):
+        ops._segments(Segments([0, 5], [0]), 4)
+    with pytest.raises(TypeError, match="Segments"):
+        ops._segments([0, 4], 4)
+
+
+def test_layouts_of_single_tokens_and_channels_are_taken_either_way():
+    one = torch.zeros(32, 32).t()[:1, :8]                        # one token, channel-first
+    assert Operators._layout(x=one) == (1, [32])
+    assert Operators._layout(x=one, base=torch.zeros(1, 6)) == (1, [32, 1])
+    assert Operators._layout(x=torch.zeros(1, 8)) == (0, [8])
+    assert Operators._layout(x=torch.zeros(5, 9)[:, 1:], base=None) == (0, [9, 0])
+    assert Operators._layout(x=torch.zeros(9, 32).t()[:5]) == (1, [32])
+    assert Operators._layout(x=torch.zeros(7, 3)[:, :1]) == (0, [3])

@@ -14,7 +14,9 @@ K82_OK, K82_ENOSPC = 0, -28
 EXPORTS = (
     "k82_create", "k82_fork", "k82_destroy", "k82_last_error", "k82_set_tensor", "k82_finalize", "k82_durations",
     "k82_decode", "k82_synthesize", "k82_reserve", "k82_pcm16", "k82_pcm16_static", "k82_set_precision", "k82_prof_enable", "k82_prof_read", "k82_debug_enable",
-    "k82_debug_info", "k82_debug_copy", "k82_debug_force", "k82_op_conv1d",
+    "k82_debug_info", "k82_debug_copy", "k82_debug_force", "k82_op_conv1d", "k82_op_lora",
+    "k82_op_lora_check", "k82_op_lora_grad", "k82_op_lora_grad_workspace", "k82_op_layernorm", "k82_op_layernorm_check",
+    "k82_op_layernorm_grad", "k82_op_layernorm_grad_workspace",
 )
 
 
@@ -27,6 +29,24 @@ class K82Config(C.Structure):
 class K82Noise(C.Structure):
     _fields_ = [("noise", C.c_void_p), ("seeds", C.c_void_p)]
 
+
+def _struct(name, *groups):
+    """ctypes.Structure with the fields of ``groups``: (ctype, "names")."""
+    return type(name, (C.Structure,), {"_fields_": [(n, t) for t, names in groups for n in names.split()]})
+
+
+_vp, _i32, _i64, _f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
+K82Segments = _struct("K82Segments", (_vp, "off index"), (_i32, "n"))
+K82Lora = _struct("K82Lora", (_i32, "dtype layout act cin cout rank adapters"), (_i64, "tokens"), (_vp, "x"), (_i64, "ldx"),
+                  (_vp, "base"), (_i64, "ldbase"), (_vp, "y"), (_i64, "ldy"), (_vp, "a b scale h"))
+K82LoraGrad = _struct("K82LoraGrad", (_i32, "dtype cin cout rank adapters"), (_i64, "tokens"), (_vp, "x"), (_i64, "ldx"),
+                      (_vp, "dy"), (_i64, "lddy"), (_vp, "h dx_base"), (_i64, "lddx_base"), (_vp, "dx"), (_i64, "lddx"),
+                      (_vp, "a b scale da db"))
+K82Layernorm = _struct("K82Layernorm", (_i32, "dtype layout c gains"), (_f32, "eps"), (_i64, "tokens"), (_vp, "x"),
+                       (_i64, "ldx"), (_vp, "res"), (_i64, "ldres"), (_vp, "y"), (_i64, "ldy"), (_vp, "gain offset mean rstd"))
+K82LayernormGrad = _struct("K82LayernormGrad", (_i32, "dtype c gains"), (_i64, "tokens"), (_vp, "x"), (_i64, "ldx"),
+                           (_vp, "res"), (_i64, "ldres"), (_vp, "dy"), (_i64, "lddy"), (_vp, "dx"), (_i64, "lddx"),
+                           (_vp, "gain mean rstd dgain doffset"))
 
 _lib = None
 
@@ -71,8 +91,14 @@ def load():
     lib.k82_debug_force.argtypes = [vp, C.c_char_p, vp, i64, i64]
     lib.k82_op_conv1d.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, i32,
                                   C.POINTER(C.c_float)]
+    for op, args in (("lora", K82Lora), ("layernorm", K82Layernorm)):
+        getattr(lib, f"k82_op_{op}").argtypes = [vp, C.POINTER(args), C.POINTER(K82Segments), vp]
+        getattr(lib, f"k82_op_{op}_check").argtypes = [C.POINTER(args), C.POINTER(K82Segments)]
+    for op, args in (("lora", K82LoraGrad), ("layernorm", K82LayernormGrad)):
+        getattr(lib, f"k82_op_{op}_grad").argtypes = [vp, C.POINTER(args), C.POINTER(K82Segments), vp, i64, vp]
+        getattr(lib, f"k82_op_{op}_grad_workspace").argtypes = [C.POINTER(args), C.POINTER(K82Segments)]
     for n in EXPORTS:
         if n != "k82_last_error":
-            getattr(lib, n).restype = C.c_int
+            getattr(lib, n).restype = i64 if n.endswith("_workspace") else C.c_int
     _lib = lib
     return lib

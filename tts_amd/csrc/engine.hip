@@ -3,6 +3,7 @@
 // conv_mfma.hip / ops.hip / source.hip on one HIP stream; no kernel is launched from anywhere
 // else.  Layout, masking and naming conventions: kernels.h.
 #include "kernels.h"
+#include "operators.h"
 #include "../../include/k82.h"
 
 #include <algorithm>
@@ -35,7 +36,7 @@ struct K82Error : std::runtime_error {
 
 inline int ru(int a, int m) { return (a + m - 1) / m * m; }
 
-std::string g_create_error;
+thread_local std::string g_create_error;      // k82_last_error(NULL): the calling thread's last create / check error
 
 // ---- k82_pcm16_static: the one entry point that allocates nothing (include/k82.h) ------------------------------
 // Staging for host -> device -> host conversion lives in a file-scope device array instead of the workspace arena.
@@ -1277,6 +1278,38 @@ template <class F> int guarded(k82_handle* h, void* stream, F&& f) {
         return K82_EINVAL;
     }
 }
+// An operator on the caller's tensors: enqueued on the caller's stream, nothing else; on the handle's own stream (stream
+// NULL) the call waits, as every other entry point does.  The thread's current device is left as it was.
+template <class F> int enqueued(k82_handle* h, void* stream, F&& f) {
+    int dev = -1;
+    (void)hipGetDevice(&dev);
+    const int rc = guarded(h, stream, [&] {
+        HIPCHK(f());
+        if (!stream) HIPCHK(hipStreamSynchronize(h->st));
+    });
+    if (dev >= 0 && h && dev != h->device) (void)hipSetDevice(dev);
+    return rc;
+}
+template <class P> void check_op(const P* p, const k82_segments* s) {
+    const std::string m = op::check(p, s);
+    REQUIRE(m.empty(), K82_EINVAL, m);
+}
+void check_workspace(int64_t need, const void* ws, int64_t bytes) {
+    REQUIRE(bytes >= need, K82_ENOSPC, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
+    REQUIRE(need == 0 || (ws && (uintptr_t)ws % 256 == 0), K82_EINVAL, "workspace must be 256-byte aligned device memory");
+}
+// the checks alone, no handle and no GPU: error text through k82_last_error(NULL)
+template <class F> int64_t checked(F&& f) {
+    try {
+        return f();
+    } catch (const K82Error& e) {
+        g_create_error = e.what();
+        return e.code;
+    } catch (const std::exception& e) {
+        g_create_error = e.what();
+        return K82_ENOMEM;
+    }
+}
 }  // namespace
 
 extern "C" {
@@ -1460,6 +1493,39 @@ int k82_pcm16_static(k82_handle* h, const float* src, int16_t* dst, int64_t n, v
         if (!ddev) HIPCHK(hipMemcpyAsync(dst, d, (size_t)n * sizeof(int16_t), hipMemcpyDeviceToHost, h->st));
         HIPCHK(hipStreamSynchronize(h->st));
         HIPCHK(hipGetLastError());
+    });
+}
+
+int k82_op_lora(k82_handle* h, const k82_lora* p, const k82_segments* seg, void* stream) {
+    return enqueued(h, stream, [&] { check_op(p, seg); return op::launch(*p, *seg, h->st); });
+}
+int k82_op_lora_check(const k82_lora* p, const k82_segments* seg) {
+    return (int)checked([&]() -> int64_t { check_op(p, seg); return K82_OK; });
+}
+int64_t k82_op_lora_grad_workspace(const k82_lora_grad* p, const k82_segments* seg) {
+    return checked([&]() -> int64_t { check_op(p, seg); return op::workspace(*p, *seg); });
+}
+int k82_op_lora_grad(k82_handle* h, const k82_lora_grad* p, const k82_segments* seg, void* workspace, int64_t workspace_bytes, void* stream) {
+    return enqueued(h, stream, [&] {
+        check_op(p, seg);
+        check_workspace(op::workspace(*p, *seg), workspace, workspace_bytes);
+        return op::launch(*p, *seg, workspace, h->st);
+    });
+}
+int k82_op_layernorm(k82_handle* h, const k82_layernorm* p, const k82_segments* seg, void* stream) {
+    return enqueued(h, stream, [&] { check_op(p, seg); return op::launch(*p, *seg, h->st); });
+}
+int k82_op_layernorm_check(const k82_layernorm* p, const k82_segments* seg) {
+    return (int)checked([&]() -> int64_t { check_op(p, seg); return K82_OK; });
+}
+int64_t k82_op_layernorm_grad_workspace(const k82_layernorm_grad* p, const k82_segments* seg) {
+    return checked([&]() -> int64_t { check_op(p, seg); return op::workspace(*p, *seg); });
+}
+int k82_op_layernorm_grad(k82_handle* h, const k82_layernorm_grad* p, const k82_segments* seg, void* workspace, int64_t workspace_bytes, void* stream) {
+    return enqueued(h, stream, [&] {
+        check_op(p, seg);
+        check_workspace(op::workspace(*p, *seg), workspace, workspace_bytes);
+        return op::launch(*p, *seg, workspace, h->st);
     });
 }
 

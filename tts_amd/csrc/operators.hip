@@ -1,0 +1,184 @@
+// Argument checks and segment tables of the operators on caller-owned tensors (operators.h): host code, no GPU needed.
+#include "operators.h"
+
+#include <algorithm>
+
+namespace op {
+namespace {
+
+// A tensor [outer][inner] with `ld` elements between rows of memory (K82_ROWS: outer = tokens, K82_COLS: channels)
+struct Span {
+    const char* p;
+    int64_t row, outer, inner;                 // bytes, rows, bytes
+    Span(const void* q, int64_t ld, int layout, int64_t tokens, int64_t c, int size)
+        : p((const char*)q), row(ld * size), outer(layout == K82_COLS ? c : tokens),
+          inner((layout == K82_COLS ? tokens : c) * size) {}
+    int64_t bytes() const { return outer > 0 ? (outer - 1) * row + inner : 0; }
+};
+bool overlap(const Span& a, const Span& b) {
+    if (!a.p || !b.p || a.bytes() == 0 || b.bytes() == 0) return false;
+    if (a.p + a.bytes() <= b.p || b.p + b.bytes() <= a.p) return false;
+    if (a.row == b.row && a.row > 0) {         // interleaved slices of one buffer
+        const int64_t m = ((b.p - a.p) % a.row + a.row) % a.row;
+        if (m >= a.inner && m + b.inner <= a.row) return false;
+    }
+    return true;
+}
+bool same(const Span& a, const Span& b) { return a.p == b.p && (a.row == b.row || a.outer <= 1); }
+
+std::string check_segments(const k82_segments* s, int64_t tokens, int lo, int hi, const char* what) {
+    if (!s) return "segments must not be NULL";
+    if (s->n < 0) return "segments: n must not be negative";
+    if (s->n == 0) return "";
+    if (!s->off || !s->index) return "segments: off and index must not be NULL";
+    if (s->off[0] < 0) return "segments: off[0] must not be negative";
+    for (int32_t i = 0; i < s->n; ++i) {
+        if (s->off[i + 1] < s->off[i]) return "segments: off must not decrease (at " + std::to_string(i) + ")";
+        if (s->index[i] < lo || s->index[i] >= hi)
+            return std::string("segments: index ") + std::to_string(s->index[i]) + " of segment " + std::to_string(i) +
+                   " is outside [" + std::to_string(lo) + ", " + what + " = " + std::to_string(hi) + ")";
+    }
+    if (s->off[s->n] > tokens)
+        return "segments: off ends at " + std::to_string(s->off[s->n]) + ", the tensors hold " + std::to_string(tokens) + " tokens";
+    return "";
+}
+std::string check_sizes(int dtype, int layout, int64_t tokens, std::initializer_list<int> channels) {
+    if (dtype != K82_F32 && dtype != K82_BF16) return "dtype must be K82_F32 or K82_BF16";
+    if (layout != K82_ROWS && layout != K82_COLS) return "layout must be K82_ROWS or K82_COLS";
+    if (layout == K82_COLS && dtype != K82_F32) return "K82_COLS exists in K82_F32 only";
+    // 32-bit token numbers in the kernels; every offset into a tensor is 64 bits wide
+    if (tokens < 0 || tokens > 0x7fff0000) return "tokens must be in [0, 2^31 - 2^16]";
+    for (int c : channels)
+        if (c < 1 || c > (1 << 20)) return "channel counts must be in [1, 2^20]";
+    return "";
+}
+std::string check_tensor(const char* name, const void* p, int64_t ld, int layout, int64_t tokens, int64_t c, int size, bool optional) {
+    if (!p) return optional || tokens == 0 ? "" : std::string(name) + " must not be NULL";
+    if ((uintptr_t)p % size) return std::string(name) + " is not aligned to its element";
+    if (ld < (layout == K82_COLS ? tokens : c)) return std::string("ld of ") + name + " is smaller than a row of it";
+    if (ld > (int64_t)1 << 40) return std::string("ld of ") + name + " is too large";
+    return "";
+}
+std::string check_lora_factors(int rank, int adapters, const void* a, const void* b, const float* scale) {
+    if (rank < 1 || rank > K82_LORA_MAX_RANK) return "rank must be in [1, 128]";
+    if (adapters < 0) return "adapters must not be negative";
+    if (adapters > 0 && (!a || !b || !scale)) return "a, b and scale must not be NULL";
+    return "";
+}
+#define OP_CHECK(e)                     \
+    do {                                \
+        const std::string m_ = (e);     \
+        if (!m_.empty()) return m_;     \
+    } while (0)
+
+}  // namespace
+
+std::string check(const k82_lora* p, const k82_segments* s) {
+    if (!p) return "arguments must not be NULL";
+    OP_CHECK(check_sizes(p->dtype, p->layout, p->tokens, {p->cin, p->cout}));
+    OP_CHECK(check_lora_factors(p->rank, p->adapters, p->a, p->b, p->scale));
+    if (p->act != K82_ACT_NONE && p->act != K82_ACT_GELU_NEW) return "act must be K82_ACT_NONE or K82_ACT_GELU_NEW";
+    OP_CHECK(check_segments(s, p->tokens, -1, p->adapters, "adapters"));
+    const int size = p->dtype == K82_F32 ? 4 : 2;
+    OP_CHECK(check_tensor("x", p->x, p->ldx, p->layout, p->tokens, p->cin, size, false));
+    OP_CHECK(check_tensor("base", p->base, p->ldbase, p->layout, p->tokens, p->cout, size, true));
+    OP_CHECK(check_tensor("y", p->y, p->ldy, p->layout, p->tokens, p->cout, size, false));
+    const Span x(p->x, p->ldx, p->layout, p->tokens, p->cin, size), y(p->y, p->ldy, p->layout, p->tokens, p->cout, size),
+        base(p->base, p->ldbase, p->layout, p->tokens, p->cout, size), h(p->h, p->rank, K82_ROWS, p->tokens, p->rank, 4);
+    if (overlap(x, y)) return "x and y overlap";
+    if (overlap(base, y) && !same(base, y)) return "base and y overlap without being one tensor";
+    if (overlap(h, x) || overlap(h, y) || overlap(h, base)) return "h overlaps another tensor";
+    return "";
+}
+std::string check(const k82_lora_grad* p, const k82_segments* s) {
+    if (!p) return "arguments must not be NULL";
+    OP_CHECK(check_sizes(p->dtype, K82_ROWS, p->tokens, {p->cin, p->cout}));
+    OP_CHECK(check_lora_factors(p->rank, p->adapters, p->a, p->b, p->scale));
+    if (p->adapters > 0 && (!p->da || !p->db)) return "da and db must not be NULL";
+    OP_CHECK(check_segments(s, p->tokens, -1, p->adapters, "adapters"));
+    const int size = p->dtype == K82_F32 ? 4 : 2;
+    OP_CHECK(check_tensor("x", p->x, p->ldx, K82_ROWS, p->tokens, p->cin, size, false));
+    OP_CHECK(check_tensor("dy", p->dy, p->lddy, K82_ROWS, p->tokens, p->cout, size, false));
+    OP_CHECK(check_tensor("h", p->h, p->rank, K82_ROWS, p->tokens, p->rank, 4, false));
+    OP_CHECK(check_tensor("dx_base", p->dx_base, p->lddx_base, K82_ROWS, p->tokens, p->cin, size, true));
+    OP_CHECK(check_tensor("dx", p->dx, p->lddx, K82_ROWS, p->tokens, p->cin, size, false));
+    const Span x(p->x, p->ldx, K82_ROWS, p->tokens, p->cin, size), dx(p->dx, p->lddx, K82_ROWS, p->tokens, p->cin, size),
+        dy(p->dy, p->lddy, K82_ROWS, p->tokens, p->cout, size), h(p->h, p->rank, K82_ROWS, p->tokens, p->rank, 4),
+        base(p->dx_base, p->lddx_base, K82_ROWS, p->tokens, p->cin, size);
+    if (overlap(dx, x) || overlap(dx, dy) || overlap(dx, h)) return "dx overlaps x, dy or h";
+    if (overlap(base, dx) && !same(base, dx)) return "dx_base and dx overlap without being one tensor";
+    return "";
+}
+std::string check(const k82_layernorm* p, const k82_segments* s) {
+    if (!p) return "arguments must not be NULL";
+    OP_CHECK(check_sizes(p->dtype, p->layout, p->tokens, {p->c}));
+    if (p->gains < 1 || !p->gain || !p->offset) return "gain and offset must hold at least one row";
+    if (!(p->eps >= 0.f)) return "eps must not be negative";
+    if (!p->mean != !p->rstd) return "mean and rstd come together";
+    OP_CHECK(check_segments(s, p->tokens, 0, p->gains, "gains"));
+    const int size = p->dtype == K82_F32 ? 4 : 2;
+    OP_CHECK(check_tensor("x", p->x, p->ldx, p->layout, p->tokens, p->c, size, false));
+    OP_CHECK(check_tensor("res", p->res, p->ldres, p->layout, p->tokens, p->c, size, true));
+    OP_CHECK(check_tensor("y", p->y, p->ldy, p->layout, p->tokens, p->c, size, false));
+    const Span x(p->x, p->ldx, p->layout, p->tokens, p->c, size), res(p->res, p->ldres, p->layout, p->tokens, p->c, size),
+        y(p->y, p->ldy, p->layout, p->tokens, p->c, size), m(p->mean, 1, K82_ROWS, p->tokens, 1, 4), r(p->rstd, 1, K82_ROWS, p->tokens, 1, 4);
+    if (overlap(x, y) && !same(x, y)) return "x and y overlap without being one tensor";
+    if (overlap(res, y) && !same(res, y)) return "res and y overlap without being one tensor";
+    if (overlap(m, r) || overlap(m, y) || overlap(r, y) || overlap(m, x) || overlap(r, x) || overlap(m, res) || overlap(r, res))
+        return "mean or rstd overlaps another tensor";
+    return "";
+}
+std::string check(const k82_layernorm_grad* p, const k82_segments* s) {
+    if (!p) return "arguments must not be NULL";
+    OP_CHECK(check_sizes(p->dtype, K82_ROWS, p->tokens, {p->c}));
+    if (p->gains < 1 || !p->gain || !p->dgain || !p->doffset) return "gain, dgain and doffset must hold at least one row";
+    if (p->tokens > 0 && (!p->mean || !p->rstd)) return "mean and rstd must not be NULL";
+    OP_CHECK(check_segments(s, p->tokens, 0, p->gains, "gains"));
+    const int size = p->dtype == K82_F32 ? 4 : 2;
+    OP_CHECK(check_tensor("x", p->x, p->ldx, K82_ROWS, p->tokens, p->c, size, false));
+    OP_CHECK(check_tensor("res", p->res, p->ldres, K82_ROWS, p->tokens, p->c, size, true));
+    OP_CHECK(check_tensor("dy", p->dy, p->lddy, K82_ROWS, p->tokens, p->c, size, false));
+    OP_CHECK(check_tensor("dx", p->dx, p->lddx, K82_ROWS, p->tokens, p->c, size, false));
+    const Span dx(p->dx, p->lddx, K82_ROWS, p->tokens, p->c, size);
+    const Span in[3] = {{p->x, p->ldx, K82_ROWS, p->tokens, p->c, size}, {p->res, p->ldres, K82_ROWS, p->tokens, p->c, size},
+                        {p->dy, p->lddy, K82_ROWS, p->tokens, p->c, size}};
+    for (const Span& v : in)
+        if (overlap(v, dx) && !same(v, dx)) return "dx overlaps an input without being one tensor with it";
+    const Span st[2] = {{p->mean, 1, K82_ROWS, p->tokens, 1, 4}, {p->rstd, 1, K82_ROWS, p->tokens, 1, 4}};
+    for (const Span& v : st)
+        if (overlap(v, dx)) return "dx overlaps mean or rstd";
+    return "";
+}
+
+std::vector<Seg> merged(const k82_segments& s) {
+    std::vector<Seg> v;
+    for (int32_t i = 0; i < s.n; ++i) {
+        const int start = (int)s.off[i], len = (int)(s.off[i + 1] - s.off[i]);
+        if (len == 0) continue;
+        if (!v.empty() && v.back().index == s.index[i]) v.back().len += len;     // (neighbours: nothing lies between them)
+        else v.push_back({start, len, s.index[i]});
+    }
+    return v;
+}
+std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile) {
+    std::vector<SegTable> out;
+    for (size_t i0 = 0; i0 < segs.size(); i0 += kSegs) {
+        out.emplace_back();
+        SegTable& t = out.back();
+        t.n = (int)std::min<size_t>(kSegs, segs.size() - i0);
+        t.tile0[0] = 0;
+        for (int i = 0; i < kSegs; ++i) {
+            if (i < t.n) {
+                const Seg& g = segs[i0 + i];
+                t.start[i] = g.start; t.len[i] = g.len; t.index[i] = g.index;
+                t.tile0[i + 1] = t.tile0[i] + (g.len - 1) / tile + 1;
+            } else {
+                t.start[i] = 0; t.len[i] = 0; t.index[i] = -1;
+                t.tile0[i + 1] = t.tile0[t.n];
+            }
+        }
+    }
+    return out;
+}
+
+}  // namespace op

@@ -15,16 +15,7 @@ import time
 import numpy as np
 
 from . import _lib, spec, weights as W
-
-
-def _cfg_struct(config):
-    pl = config["plbert"]
-    return _lib.K82Config(
-        n_token=config["n_token"], hidden_dim=config["hidden_dim"], style_dim=config["style_dim"],
-        n_layer=config["n_layer"], max_dur=config["max_dur"], text_kernel=config["text_encoder_kernel_size"],
-        bert_hidden=pl["hidden_size"], bert_heads=pl["num_attention_heads"], bert_inter=pl["intermediate_size"],
-        bert_layers=pl["num_hidden_layers"], bert_max_pos=pl["max_position_embeddings"],
-        bert_embed=spec.ALBERT_EMBED)
+from .operators import Operators, _cfg_struct  # noqa: F401
 
 
 def _ptr(a):
@@ -49,11 +40,10 @@ def _host_buffer(n):
     return np.empty((n,), dtype=np.float32)
 
 
-class Engine:
+class Engine(Operators):
     """Kokoro-82M on one MI355X.  ``state_dicts``: the 5 raw checkpoint state dicts."""
 
     def __init__(self, state_dicts, config=None, device=0, precision="fp32"):
-        self.lib = _lib.load()
         # k82_durations leaves the token-rate state of ITS batch inside the handle for k82_decode, so the pair is one
         # critical section: every caller that may share this Engine with another thread (both front doors do, and the
         # reference runs two pool threads on one Kokoro object: epubviewer_06_latest_1_nov_2025_theme.py:407,692,715)
@@ -63,13 +53,9 @@ class Engine:
         self._pending = None               # (owner thread id, n_frames) of the durations call a decode may follow
         self.config = config or spec.DEFAULT_CONFIG
         self.device = device
-        self.h = C.c_void_p()
         self._parent = None                # Engine.fork(): the engine whose weights this one reads
         self._forks = []
-        cfg = _cfg_struct(self.config)
-        rc = self.lib.k82_create(C.byref(cfg), device, C.byref(self.h))
-        if rc != 0:
-            raise RuntimeError(f"k82_create failed ({rc}): {self.lib.k82_last_error(None).decode()}")
+        self._open(self.config)
         flat = W.fold_state_dicts(state_dicts, self.config)
         for name, arr in flat.items():
             arr = np.ascontiguousarray(arr, dtype=np.float32)
@@ -127,13 +113,6 @@ class Engine:
             self._reserved = (max(want[0], have[0]), max(want[1], have[1]))
 
     # ------------------------------------------------------------------ plumbing
-    def _check(self, rc):
-        if rc != 0:
-            msg = self.lib.k82_last_error(self.h).decode()
-            if rc in (-22, -28):
-                raise ValueError(f"k82 error {rc}: {msg}")
-            raise RuntimeError(f"k82 error {rc}: {msg}")
-
     def close(self):
         if getattr(self, "h", None) and self.h.value:
             for f in list(getattr(self, "_forks", ())):      # forks read this engine's weights: they go first
