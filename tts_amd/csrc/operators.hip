@@ -46,8 +46,8 @@ std::string check_sizes(int dtype, int layout, int64_t tokens, std::initializer_
     if (dtype != K82_F32 && dtype != K82_BF16) return "dtype must be K82_F32 or K82_BF16";
     if (layout != K82_ROWS && layout != K82_COLS) return "layout must be K82_ROWS or K82_COLS";
     if (layout == K82_COLS && dtype != K82_F32) return "K82_COLS exists in K82_F32 only";
-    // 32-bit token numbers in the kernels; every offset into a tensor is 64 bits wide
-    if (tokens < 0 || tokens > 0x7fff0000) return "tokens must be in [0, 2^31 - 2^16]";
+    // a launch may need 256 threads for a token and holds less than 2^32; every offset into a tensor is 64 bits wide
+    if (tokens < 0 || tokens >= 1 << 24) return "tokens must be in [0, 2^24)";
     for (int c : channels)
         if (c < 1 || c > (1 << 20)) return "channel counts must be in [1, 2^20]";
     return "";
@@ -179,6 +179,47 @@ std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile) {
         }
     }
     return out;
+}
+
+RunPlan runs(const k82_segments& s, int indices, int rows) {
+    std::vector<Seg> v = merged(s);
+    v.erase(std::remove_if(v.begin(), v.end(), [](const Seg& g) { return g.index < 0; }), v.end());
+    std::stable_sort(v.begin(), v.end(), [](const Seg& a, const Seg& b) { return a.index < b.index; });
+    RunPlan plan;
+    std::vector<int> count(indices + 1, 0);    // chunks of each index
+    for (size_t i0 = 0; i0 < v.size(); i0 += kSegs) {
+        plan.tables.emplace_back();
+        RunTable& t = plan.tables.back();
+        t.pieces = (int)std::min<size_t>(kSegs, v.size() - i0);
+        t.runs = 0; t.rows = rows;
+        t.cum[0] = 0;
+        for (int i = 0; i < t.pieces; ++i) {
+            const Seg& g = v[i0 + i];
+            if (i == 0 || g.index != t.index[t.runs - 1]) { t.index[t.runs] = g.index; t.run_cum[t.runs++] = t.cum[i]; }
+            t.start[i] = g.start;
+            t.cum[i + 1] = t.cum[i] + g.len;
+        }
+        t.run_cum[t.runs] = t.cum[t.pieces];
+        t.chunk0[0] = plan.chunks;
+        for (int r = 0; r < t.runs; ++r) {
+            const int n = (t.run_cum[r + 1] - t.run_cum[r] - 1) / rows + 1;
+            t.chunk0[r + 1] = t.chunk0[r] + n;
+            count[t.index[r]] += n;
+        }
+        plan.chunks = t.chunk0[t.runs];
+        for (int i = t.pieces; i < kSegs; ++i) { t.start[i] = 0; t.cum[i + 1] = t.cum[t.pieces]; }
+        for (int i = t.runs; i < kSegs; ++i) { t.index[i] = 0; t.run_cum[i + 1] = t.run_cum[t.runs]; t.chunk0[i + 1] = t.chunk0[t.runs]; }
+    }
+    for (int b = 0, first = 0; b < indices; b += kSegs) {
+        plan.reduce.emplace_back();
+        ReduceTable& t = plan.reduce.back();
+        t.base = b;
+        t.n = std::min(kSegs, indices - b);
+        t.first[0] = first;
+        for (int i = 0; i < kSegs; ++i) t.first[i + 1] = t.first[i] + (i < t.n ? count[b + i] : 0);
+        first = t.first[t.n];
+    }
+    return plan;
 }
 
 }  // namespace op
