@@ -105,6 +105,108 @@ __global__ __launch_bounds__(kThreads<W>) void norm_rows_kernel(SegTable sg, k82
     }
 }
 
+// Channel-first rows (the engine's layout).  A workgroup of NW waves holds 4 Q tokens: a lane has four of them (16 bytes) of
+// every STEP-th channel, a wave's load covers 64 / Q channels.  Tiles lie on the token grid of the tensor, not of the
+// sentences: rows start on lines and a batch of short sentences fills its tiles; the gain row is picked by token where a tile
+// holds several sentences.  The shape goes by the channel count alone, so a token's bits do not depend on its batch.
+// 32 tokens are the 128 bytes of a line: 16411 x 768 with a residual 46 us (3.3 TB/s; token rows: 34 us); 64 tokens 51 us and
+// 16 tokens 50 to 56 us.  All of a tile is loaded, then all of it stored, which two workgroups on a CU overlap only in part.
+constexpr int kColsMax = 4096;                 // channels that fit
+template <int Q, int NW, int NV> __global__ __launch_bounds__(64 * NW) void norm_cols_kernel(SegTable sg, k82_layernorm p) {
+    constexpr int TOK = 4 * Q, STEP = NW * 64 / Q;               // tokens of a tile, channels of a round
+    __shared__ float4 red[2][NW][Q];
+    __shared__ int kind[TOK];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quad = lane & (Q - 1);
+    const int first = sg.start[0], end = first + sg.tile0[sg.n];
+    const int t0 = (first & ~(TOK - 1)) + (int)blockIdx.x * TOK + 4 * quad, c0 = 64 / Q * wave + lane / Q;
+    const bool whole = t0 >= first && t0 + 4 <= end;
+    if (threadIdx.x < TOK) {
+        const int t = min(max((first & ~(TOK - 1)) + (int)blockIdx.x * TOK + (int)threadIdx.x, first), end - 1) - first;
+        int s = 0;
+        for (int step = op::kSegs / 2; step > 0; step >>= 1)     // last segment that starts at or before t
+            if (s + step < sg.n && sg.tile0[s + step] <= t) s += step;
+        kind[threadIdx.x] = sg.index[s];
+    }
+    auto fetch = [&](const void* q, int64_t ld, int c) -> float4 {
+        const float* v = (const float*)q + (int64_t)c * ld + t0;
+        if (whole) { const raw4 r = *(const raw4_f*)v; return make_float4(__uint_as_float(r[0]), __uint_as_float(r[1]), __uint_as_float(r[2]), __uint_as_float(r[3])); }
+        auto at = [&](int j) { return t0 + j >= first && t0 + j < end ? v[j] : 0.f; };
+        return make_float4(at(0), at(1), at(2), at(3));
+    };
+    float4 z[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) z[i] = c0 + STEP * i < p.c ? fetch(p.x, p.ldx, c0 + STEP * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.res) {
+        float4 r[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) r[i] = c0 + STEP * i < p.c ? fetch(p.res, p.ldres, c0 + STEP * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) z[i] = make_float4(z[i].x + r[i].x, z[i].y + r[i].y, z[i].z + r[i].z, z[i].w + r[i].w);
+    }
+    // sum over the channels: the lane's own, the four of a wave, the 16 waves
+    auto total = [&](float4 v, float4 (&buf)[NW][Q]) -> float4 {
+        float a[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int m = Q; m < 64; m *= 2)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] += __shfl_xor(a[j], m, 64);
+        if (lane < Q) buf[wave][quad] = make_float4(a[0], a[1], a[2], a[3]);
+        __syncthreads();
+        float4 s = buf[0][quad];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) {
+            const float4 b = buf[w][quad];
+            s = make_float4(s.x + b.x, s.y + b.y, s.z + b.z, s.w + b.w);
+        }
+        return s;
+    };
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) s = make_float4(s.x + z[i].x, s.y + z[i].y, s.z + z[i].z, s.w + z[i].w);
+    s = total(s, red[0]);
+    const float4 mean = make_float4(s.x / p.c, s.y / p.c, s.z / p.c, s.w / p.c);
+    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (c0 + STEP * i < p.c) {
+            z[i] = make_float4(z[i].x - mean.x, z[i].y - mean.y, z[i].z - mean.z, z[i].w - mean.w);
+            q = make_float4(fmaf(z[i].x, z[i].x, q.x), fmaf(z[i].y, z[i].y, q.y), fmaf(z[i].z, z[i].z, q.z), fmaf(z[i].w, z[i].w, q.w));
+        }
+    }
+    q = total(q, red[1]);
+    const float4 rstd = make_float4(1.0f / sqrtf(q.x / p.c + p.eps), 1.0f / sqrtf(q.y / p.c + p.eps),
+                                    1.0f / sqrtf(q.z / p.c + p.eps), 1.0f / sqrtf(q.w / p.c + p.eps));
+    auto store = [&](float* v, float4 y) {
+        if (whole) { *(raw4_f*)v = raw4{__float_as_uint(y.x), __float_as_uint(y.y), __float_as_uint(y.z), __float_as_uint(y.w)}; return; }
+        const float a[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (t0 + j >= first && t0 + j < end) v[j] = a[j];
+    };
+    if (p.mean && c0 == 0) { store(p.mean + t0, mean); store(p.rstd + t0, rstd); }
+    const float *gain = (const float*)p.gain, *offset = (const float*)p.offset;
+    const int k0 = kind[4 * quad], k1 = kind[4 * quad + 1], k2 = kind[4 * quad + 2], k3 = kind[4 * quad + 3];
+    const bool uniform = __all(k0 == kind[0] && k1 == kind[0] && k2 == kind[0] && k3 == kind[0]);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = c0 + STEP * i;
+        if (c >= p.c) continue;
+        float4 g, o;
+        const int64_t at = (int64_t)k0 * p.c + c;
+        g.x = gain[at]; o.x = offset[at];
+        if (uniform) {
+            g = make_float4(g.x, g.x, g.x, g.x);
+            o = make_float4(o.x, o.x, o.x, o.x);
+        } else {
+            const int64_t a1 = (int64_t)k1 * p.c + c, a2 = (int64_t)k2 * p.c + c, a3 = (int64_t)k3 * p.c + c;
+            g = make_float4(g.x, gain[a1], gain[a2], gain[a3]);
+            o = make_float4(o.x, offset[a1], offset[a2], offset[a3]);
+        }
+        store((float*)p.y + (int64_t)c * p.ldy + t0, make_float4(fmaf(z[i].x * rstd.x, g.x, o.x), fmaf(z[i].y * rstd.y, g.y, o.y),
+                                                                 fmaf(z[i].z * rstd.z, g.z, o.z), fmaf(z[i].w * rstd.w, g.w, o.w)));
+    }
+}
+
 template <int N> __device__ __forceinline__ float block_total(float v, float (&sh)[N]) {    // 64 N threads
     v = wave_total(v);
     __syncthreads();
@@ -116,7 +218,7 @@ template <int N> __device__ __forceinline__ float block_total(float v, float (&s
     return s;
 }
 
-// Rows that no registers hold, and channel-first tensors: one workgroup per token, the row read three times.
+// Rows that no registers hold: one workgroup per token, the row read three times.
 template <class T>
 __global__ __launch_bounds__(256) void norm_token_kernel(SegTable sg, k82_layernorm p, int64_t xt, int64_t xc, int64_t rt, int64_t rc, int64_t yt, int64_t yc) {
     __shared__ float sh[4];
@@ -314,6 +416,18 @@ template <class T> hipError_t forward(const k82_layernorm& p, const k82_segments
     const bool cols = p.layout == K82_COLS;
     for (const SegTable& t : op::tables(op::merged(s), 1)) {
         const int tokens = t.tile0[t.n];
+        if (cols && p.c <= kColsMax) {
+            auto go = [&](auto q, auto w, auto v) {
+                constexpr int Q = decltype(q)::value, NW = decltype(w)::value;
+                const int tiles = (t.start[0] + tokens - 1) / (4 * Q) - t.start[0] / (4 * Q) + 1;
+                return op::run(norm_cols_kernel<Q, NW, decltype(v)::value>, dim3(tiles), dim3(64 * NW), 0, st, t, p);
+            };
+            const std::integral_constant<int, 12> v12; const std::integral_constant<int, 2> q2; const std::integral_constant<int, 4> q4; const std::integral_constant<int, 8> q8;
+            const std::integral_constant<int, 16> w16;
+            OP_TRY(p.c <= 256 ? go(q8, q8, q4) : p.c <= 512 ? go(q8, q8, q8) : p.c <= 768 ? go(q8, q8, v12) :
+                   p.c <= 1536 ? go(q8, w16, v12) : p.c <= 2048 ? go(q4, w16, q8) : go(q2, w16, q8));
+            continue;
+        }
         if (cols || p.c > kRowMax) {
             OP_TRY(op::run(norm_token_kernel<T>, dim3(tokens), dim3(256), 0, st, t, p, cols ? 1 : p.ldx, cols ? p.ldx : 1,
                            cols ? 1 : p.ldres, cols ? p.ldres : 1, cols ? 1 : p.ldy, cols ? p.ldy : 1));

@@ -83,6 +83,7 @@ typedef uint16_t bf16_t;
 typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
 // 16 bytes at any address of the element's own alignment: one global_load_dwordx4 / store (the target reads unaligned)
 typedef raw4 raw4_any __attribute__((aligned(2)));
+typedef raw4 raw4_f __attribute__((aligned(4)));
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(bf16_t v) { return __uint_as_float((uint32_t)v << 16); }
