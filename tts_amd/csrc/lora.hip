@@ -31,196 +31,298 @@ template <> __device__ __forceinline__ f4 product<float>(raw4 a, raw4 b, f4 c) {
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
     return c;
 }
-// h as the second product's operand.  f32: itself.  bf16: the 8 places of a lane hold the four values in two parts, and B's
-// four values come twice: h = hi + lo to 2^-16 at the price of one instruction (rounded to one part alone, h would cost
-// half of the result's own precision).
-template <class T> __device__ __forceinline__ raw4 second(f4 h);
-template <> __device__ __forceinline__ raw4 second<float>(f4 h) { return __builtin_bit_cast(raw4, h); }
-template <> __device__ __forceinline__ raw4 second<bf16_t>(f4 h) {
-    raw4 r;
-    r[0] = bf16_pair(h[0], h[1]);
-    r[1] = bf16_pair(h[2], h[3]);
-    r[2] = bf16_pair(h[0] - __uint_as_float(r[0] << 16), h[1] - __uint_as_float(r[0] & 0xffff0000u));
-    r[3] = bf16_pair(h[2] - __uint_as_float(r[1] << 16), h[3] - __uint_as_float(r[1] & 0xffff0000u));
-    return r;
+// Operands reach the matrix units through LDS: a wave reads 16 rows x 64 bytes with four neighbouring lanes on each row (16
+// requests to the cache; a lane a row, as the instruction wants it, would be 64), and takes them from LDS in the instruction's
+// order.  The 16-byte places of a row are turned by row / 4, so neither side meets a bank twice.  The region belongs to one
+// wave, whose LDS accesses happen in order: no barrier.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
-// four values of a row of B from p on, n of them inside, in the form that second() needs
-__device__ __forceinline__ raw4 factor4(const float* p, int n) { return n <= 0 ? raw4{0u, 0u, 0u, 0u} : load_part(p, n); }
-__device__ __forceinline__ raw4 factor4(const bf16_t* p, int n) {
-    raw2 r = {0u, 0u};
-    if (n >= 4) r = *(const raw2_any*)p;
-    else
+template <class T> __device__ __forceinline__ raw4 grab(const T* p, int n) { return n > 0 ? load_part(p, n) : raw4{0u, 0u, 0u, 0u}; }
+__device__ __forceinline__ void put_tile(raw4* tile, raw4 v) {
+    const int lane = threadIdx.x & 63;
+    tile[(lane & ~3) + ((lane & 3) ^ (lane >> 4))] = v;
+}
+__device__ __forceinline__ raw4 get_tile(const raw4* tile) {
+    const int col = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    return tile[4 * col + (g ^ (col >> 2))];
+}
+
+// The factor rank in tiles: RT of 16 rows.  From two on, bf16 pairs them so that a lane's h are 8 consecutive ranks: row m of
+// tile 2 j + e is the rank 32 j + 8 (m / 4) + 4 e + m % 4.
+template <class T, int RT> __device__ __forceinline__ int rank_of(int tile, int row) {
+    if constexpr (Vec<T>::N == 8 && RT > 1) return 32 * (tile >> 1) + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3);
+    return 16 * tile + row;
+}
+// h as the second product's operand, and that product of one row tile of B with one tile of tokens.
+// f32: itself.  bf16: in two parts, h = hi + lo to 2^-16 (rounded to one part alone, h would cost half of the result's own
+// precision); at one tile both parts share an instruction, with B's four values twice.
+template <class T, int RT> struct Second;
+template <int RT> struct Second<float, RT> {
+    static constexpr int CHUNKS = RT;          // 64-byte chunks of a row of B
+    raw4 v[RT];
+    __device__ __forceinline__ void set(const f4 (&h)[RT]) {
 #pragma unroll
-        for (int j = 0; j < 3; ++j)
-            if (j < n) r[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
-    return raw4{r[0], r[1], r[0], r[1]};
+        for (int r = 0; r < RT; ++r) v[r] = __builtin_bit_cast(raw4, h[r]);
+    }
+    __device__ __forceinline__ f4 times(const raw4 (&b)[CHUNKS], f4 d) const {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) d = product<float>(b[r], v[r], d);
+        return d;
+    }
+};
+template <int RT> struct Second<bf16_t, RT> {
+    static constexpr int CHUNKS = (RT + 1) / 2;
+    raw4 v[RT];                                // RT = 1: hi | lo; else hi and lo of each pair
+    static __device__ __forceinline__ void parts(const f4& h, uint32_t* hi, uint32_t* lo) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            hi[j] = bf16_pair(h[2 * j], h[2 * j + 1]);
+            lo[j] = bf16_pair(h[2 * j] - __uint_as_float(hi[j] << 16), h[2 * j + 1] - __uint_as_float(hi[j] & 0xffff0000u));
+        }
+    }
+    __device__ __forceinline__ void set(const f4 (&h)[RT]) {
+        uint32_t hi[RT][2], lo[RT][2];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) parts(h[r], hi[r], lo[r]);
+        if constexpr (RT == 1) v[0] = raw4{hi[0][0], hi[0][1], lo[0][0], lo[0][1]};
+        else
+#pragma unroll
+            for (int r = 0; r < RT; r += 2) {
+                v[r] = raw4{hi[r][0], hi[r][1], hi[r + 1][0], hi[r + 1][1]};
+                v[r + 1] = raw4{lo[r][0], lo[r][1], lo[r + 1][0], lo[r + 1][1]};
+            }
+    }
+    __device__ __forceinline__ f4 times(const raw4 (&b)[CHUNKS], f4 d) const {
+        if constexpr (RT == 1) return product<bf16_t>(b[0], v[0], d);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) d = product<bf16_t>(b[r >> 1], v[r], d);
+        return d;
+    }
+};
+// a row tile of B from LDS: chunk j as times() takes it
+template <class T, int RT> __device__ __forceinline__ raw4 get_factor(const raw4* tile) {
+    if constexpr (Vec<T>::N == 8 && RT == 1) {                   // ranks 4 g .. 4 g + 3, twice
+        const int col = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+        const raw2 r = ((const raw2*)(tile + 4 * col + ((g >> 1) ^ (col >> 2))))[g & 1];
+        return raw4{r[0], r[1], r[0], r[1]};
+    } else return get_tile(tile);
 }
 
-constexpr int kWaves = 4;
-
-// The sum over the waves' parts of k, and what follows from it for every wave: h for the second product, and h itself if kept
-template <class T, int RT, int TT> struct Shared { f4 part[kWaves][RT * TT][64]; };
-template <class T, int RT, int TT>
-__device__ __forceinline__ void join(Shared<T, RT, TT>& sh, f4 (&acc)[RT][TT], raw4 (&h)[RT][TT], int rank, float scale, float* keep, const int64_t* tok, const bool* in) {
+// The sum over the waves' parts of k, and what follows from it for every wave: h for the second product, and h itself if kept.
+// tok: the token of this lane's column.
+template <class T, int NW, int RT, int TT>
+__device__ __forceinline__ void join(f4 (*part)[RT * TT][64], f4 (&acc)[RT][TT], Second<T, RT> (&h)[TT], int rank, float scale, float* keep, const int64_t* tok, const bool* in) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int t = 0; t < TT; ++t) sh.part[wave][r * TT + t][lane] = acc[r][t];
+        for (int t = 0; t < TT; ++t) part[wave][r * TT + t][lane] = acc[r][t];
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int t = 0; t < TT; ++t) {
+        f4 sum[RT];
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
+        for (int r = 0; r < RT; ++r) {
             const int i = r * TT + t;
-            f4 v = (sh.part[0][i][lane] + sh.part[1][i][lane]) + (sh.part[2][i][lane] + sh.part[3][i][lane]);
-            const int r0 = 16 * r + 4 * g;
+            f4 v = part[0][i][lane];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) v += part[w][i][lane];
+            const int r0 = rank_of<T, RT>(r, 4 * g);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (r0 + j >= rank) v[j] = 0.f;                  // rows of A behind the rank were read from its last row
-            if (keep && wave == i % kWaves && in[t]) {
+            if (keep && wave == i % NW && in[t]) {
                 float* q = keep + tok[t] * rank + r0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (r0 + j < rank) q[j] = v[j];
             }
-            h[r][t] = second<T>(v * scale);
+            sum[r] = v * scale;
         }
+        h[t].set(sum);
+    }
+    __syncthreads();                                             // the parts' memory is used again
 }
 
-// Token rows.  A workgroup takes 16 TT tokens of a segment; its waves share the k of the first product (each takes every fourth
-// 64 bytes of a row, so the four read 256 contiguous bytes) and the output channels of the second.  blockIdx.y splits the
-// output channels where there are few tokens; each part then computes h for itself, from cache.
-template <class T, int RT, int TT>
-__global__ __launch_bounds__(64 * kWaves) void lora_rows_kernel(SegTable sg, k82_lora p) {
-    constexpr int V = Vec<T>::N, K = 4 * V, U = RT * TT >= 8 ? 2 : 4;            // U: steps whose loads are in flight together
-    __shared__ Shared<T, RT, TT> sh;
+constexpr int most(int a, int b) { return a > b ? a : b; }
+constexpr int kPad = 4;                        // floats behind a row of the results' tile: rows start on different banks
+
+// Token rows.  A workgroup takes 16 TT tokens of a segment; its NW waves share the k of the first product (each takes every
+// NW-th 64 bytes of a row, so together they read 64 NW contiguous bytes) and the output channels of the second, 128 bytes of a
+// row a wave at a time.  The results cross LDS once more, so that base and y are read and written in whole lines.
+// blockIdx.y splits the output channels where there are few tokens; each part then computes h for itself, from cache.
+template <class T, int NW, int RT, int TT>
+__global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lora p) {
+    constexpr int V = Vec<T>::N, K = 4 * V, U = RT + TT > 4 ? 2 : 4;             // U: steps whose loads are in flight together
+    constexpr int CH = 8 * V, MT = CH / 16, CK = Second<T, RT>::CHUNKS;          // channels, row tiles of B, chunks of a row of B
+    constexpr int kTiles = most(RT + TT, MT * CK), kRow = CH + kPad;
+    constexpr int kOwn = most(kTiles * 1024, MT * CK * 1024 + 16 * kRow * 4);    // a wave's own bytes
+    __shared__ __align__(16) char lds[most(NW * kOwn, NW * RT * TT * 1024)];
     const int s = seg_of(sg, blockIdx.x), k = sg.index[s];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     if (k < 0 && p.act == K82_ACT_NONE && p.base == p.y && !p.h) return;
-    int64_t tok[TT];
-    bool in[TT];
-    const int row0 = ((int)blockIdx.x - sg.tile0[s]) * 16 * TT;
+    raw4* own = (raw4*)(lds + wave * kOwn);
+    float* result = (float*)(own + MT * CK * 64);
+    const int row0 = ((int)blockIdx.x - sg.tile0[s]) * 16 * TT, last = sg.len[s] - 1;
+    const int64_t t0 = sg.start[s];
+    // Second product: this lane's 16 bytes of rows (lane / 8) + 8 i of the tokens
+    const int blocks = (p.cout + CH - 1) / CH, stride = NW * gridDim.y;
+    int blk = (int)blockIdx.y * NW + wave;
+    raw4 base[2 * TT], fac[MT * CK];
+    const T* b = (const T*)p.b + (int64_t)max(k, 0) * p.cout * p.rank;
+    auto fetch = [&](int blk) {
+        const int c = blk * CH + V * (lane & 7);
+        if (p.base) {
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        const int i = row0 + 16 * t + col;
-        in[t] = i < sg.len[s];
-        tok[t] = sg.start[s] + min(i, sg.len[s] - 1);
-    }
-    f4 acc[RT][TT];
-    raw4 h[RT][TT];
+            for (int i = 0; i < 2 * TT; ++i) base[i] = grab((const T*)p.base + (t0 + min(row0 + 8 * i + (lane >> 3), last)) * p.ldbase + c, p.cout - c);
+        }
+        if (k >= 0) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+            for (int m = 0; m < MT; ++m) {
+                const T* q = b + (int64_t)min(blk * CH + 16 * m + (lane >> 2), p.cout - 1) * p.rank + V * (lane & 3);
 #pragma unroll
-        for (int t = 0; t < TT; ++t) { acc[r][t] = f4{0.f, 0.f, 0.f, 0.f}; h[r][t] = raw4{0u, 0u, 0u, 0u}; }
+                for (int c = 0; c < CK; ++c) fac[m * CK + c] = grab(q + c * K, p.rank - c * K - V * (lane & 3));
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 2 * TT; ++i) base[i] = raw4{0u, 0u, 0u, 0u};
+    if (blk < blocks) fetch(blk);
+    Second<T, RT> h[TT];
     if (k >= 0) {
+        f4 acc[RT][TT];
         const T *a[RT], *x[TT];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) a[r] = (const T*)p.a + ((int64_t)k * p.rank + min(16 * r + col, p.rank - 1)) * p.cin + g * V;
+        for (int r = 0; r < RT; ++r) a[r] = (const T*)p.a + ((int64_t)k * p.rank + min(rank_of<T, RT>(r, lane >> 2), p.rank - 1)) * p.cin + V * (lane & 3);
 #pragma unroll
-        for (int t = 0; t < TT; ++t) x[t] = (const T*)p.x + tok[t] * p.ldx + g * V;
+        for (int t = 0; t < TT; ++t) x[t] = (const T*)p.x + (t0 + min(row0 + 16 * t + (lane >> 2), last)) * p.ldx + V * (lane & 3);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[r][t] = f4{0.f, 0.f, 0.f, 0.f};
+        auto multiply = [&](const raw4 (&fa)[RT], const raw4 (&fx)[TT]) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fa[r]);
+#pragma unroll
+            for (int t = 0; t < TT; ++t) put_tile(own + (RT + t) * 64, fx[t]);
+            wave_fence();
+            raw4 ta[RT], tx[TT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) ta[r] = get_tile(own + r * 64);
+#pragma unroll
+            for (int t = 0; t < TT; ++t) tx[t] = get_tile(own + (RT + t) * 64);
+            wave_fence();
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) acc[r][t] = product<T>(ta[r], tx[t], acc[r][t]);
+        };
         const int full = p.cin / K;
         auto steps = [&](int i0, auto n) {
             constexpr int n_ = decltype(n)::value;
             raw4 fa[n_][RT], fx[n_][TT];
 #pragma unroll
             for (int i = 0; i < n_; ++i) {
-                const int at = (i0 + i * kWaves) * K;
+                const int at = (i0 + i * NW) * K;
 #pragma unroll
                 for (int t = 0; t < TT; ++t) fx[i][t] = *(const raw4_any*)(x[t] + at);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) fa[i][r] = *(const raw4_any*)(a[r] + at);
             }
 #pragma unroll
-            for (int i = 0; i < n_; ++i)
-#pragma unroll
-                for (int r = 0; r < RT; ++r)
-#pragma unroll
-                    for (int t = 0; t < TT; ++t) acc[r][t] = product<T>(fa[i][r], fx[i][t], acc[r][t]);
+            for (int i = 0; i < n_; ++i) multiply(fa[i], fx[i]);
         };
         int i = wave;
-        for (; i + (U - 1) * kWaves < full; i += U * kWaves) steps(i, std::integral_constant<int, U>());
-        for (; i < full; i += kWaves) steps(i, std::integral_constant<int, 1>());
+        for (; i + (U - 1) * NW < full; i += U * NW) steps(i, std::integral_constant<int, U>());
+        if (U > 2 && i + NW < full) { steps(i, std::integral_constant<int, 2>()); i += 2 * NW; }
+        if (i < full) { steps(i, std::integral_constant<int, 1>()); i += NW; }
         if (i == full && p.cin % K) {                            // one wave: the end of the row, zeros behind it
-            const int at = full * K, n = p.cin - at - g * V;
+            const int at = full * K, n = p.cin - at - V * (lane & 3);
             raw4 fa[RT], fx[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) fx[t] = n > 0 ? load_part(x[t] + at, n) : raw4{0u, 0u, 0u, 0u};
+            for (int t = 0; t < TT; ++t) fx[t] = grab(x[t] + at, n);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) fa[r] = n > 0 ? load_part(a[r] + at, n) : raw4{0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int t = 0; t < TT; ++t) acc[r][t] = product<T>(fa[r], fx[t], acc[r][t]);
+            for (int r = 0; r < RT; ++r) fa[r] = grab(a[r] + at, n);
+            multiply(fa, fx);
         }
-        join<T, RT, TT>(sh, acc, h, p.rank, p.scale[k], blockIdx.y == 0 ? p.h : nullptr, tok, in);
+        int64_t tok[TT];
+        bool in[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) { tok[t] = t0 + row0 + 16 * t + col; in[t] = row0 + 16 * t + col <= last; }
+        join<T, NW, RT, TT>((f4(*)[RT * TT][64])lds, acc, h, p.rank, p.scale[k], blockIdx.y == 0 ? p.h : nullptr, tok, in);
     } else if (p.h && blockIdx.y == 0) {
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
-            if (in[t])
-                for (int r = 4 * wave + g; r < p.rank; r += 4 * kWaves) p.h[tok[t] * p.rank + r] = 0.f;
+        const int n = min(16 * TT, last + 1 - row0) * p.rank;
+        for (int i = threadIdx.x; i < n; i += 64 * NW) p.h[(t0 + row0) * p.rank + i] = 0.f;
     }
-    // Second product: V consecutive channels a lane (16 bytes of y), 4 V a block of the wave: the rows of B behind the 16 rows of
-    // instruction j are the channels V (row / 4) + 4 j + row % 4.
-    constexpr int J = V / 4;
-    const T* b = (const T*)p.b + (int64_t)max(k, 0) * p.cout * p.rank;
-    const int blocks = (p.cout + K - 1) / K;
-    for (int blk = 2 * ((int)blockIdx.y * kWaves + wave); blk < blocks; blk += 2 * kWaves * gridDim.y) {
+    for (; blk < blocks; blk += stride) {
+        raw4 now[2 * TT], tile[MT][CK];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int c0 = (blk + half) * K, mine = c0 + g * V, n = p.cout - mine;
-            if (c0 >= p.cout) break;
-            f4 d[TT][J];
+        for (int i = 0; i < 2 * TT; ++i) now[i] = base[i];
+        if (k >= 0) {
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                raw4 v = {0u, 0u, 0u, 0u};
-                if (p.base && n > 0) v = load_part((const T*)p.base + tok[t] * p.ldbase + mine, n);
-                float f[V];
-                Vec<T>::unpack(v, f);
+            for (int i = 0; i < MT * CK; ++i) put_tile(own + i * 64, fac[i]);
+            wave_fence();
 #pragma unroll
-                for (int j = 0; j < J; ++j) d[t][j] = f4{f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]};
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int c = 0; c < CK; ++c) tile[m][c] = get_factor<T, RT>(own + (m * CK + c) * 64);
+        }
+        if (blk + stride < blocks) fetch(blk + stride);          // the next block is on its way while this one is multiplied
+        const int c = blk * CH + V * (lane & 7), n = p.cout - c;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            if (k >= 0) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) *(f4*)(result + col * kRow + 16 * m + 4 * g) = h[t].times(tile[m], f4{0.f, 0.f, 0.f, 0.f});
+                wave_fence();
             }
-            if (k >= 0)
 #pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const T* q = b + (int64_t)min(c0 + V * (col >> 2) + 4 * j + (col & 3), p.cout - 1) * p.rank + 4 * g;
+            for (int i = 0; i < 2; ++i) {
+                float f[V];
+                Vec<T>::unpack(now[2 * t + i], f);
+                if (k >= 0) {
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        const raw4 f = factor4(q + 16 * r, p.rank - 16 * r - 4 * g);
-#pragma unroll
-                        for (int t = 0; t < TT; ++t) d[t][j] = product<T>(f, h[r][t], d[t][j]);
+                    for (int j = 0; j < V; j += 4) {
+                        const f4 d = *(const f4*)(result + (8 * i + (lane >> 3)) * kRow + V * (lane & 7) + j);
+                        f[j] += d[0]; f[j + 1] += d[1]; f[j + 2] += d[2]; f[j + 3] += d[3];
                     }
                 }
-#pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                float f[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) f[j] = d[t][j >> 2][j & 3];
                 if (p.act == K82_ACT_GELU_NEW)
 #pragma unroll
                     for (int j = 0; j < V; ++j) f[j] = op_gelu_new(f[j]);
-                if (in[t] && n > 0) store_part((T*)p.y + tok[t] * p.ldy + mine, f, n);
+                const int row = row0 + 16 * t + 8 * i + (lane >> 3);
+                if (row <= last && n > 0) store_part((T*)p.y + (t0 + row) * p.ldy + c, f, n);
             }
+            wave_fence();
         }
     }
 }
 
 // Channel-first: the same products, TT consecutive tokens a lane (tile t of a lane's tokens is TT col + t), 16 TT tokens a
-// workgroup, on the token grid of the tensor.  A tile that holds several segments is walked once for each.
-template <int TT> __device__ __forceinline__ void load_tokens(float (&v)[TT], const float* p, int64_t t, int64_t lo, int64_t hi) {
-    if (t >= lo && t + TT <= hi) {
-        if constexpr (TT == 4) { const raw4 r = *(const raw4_f*)(p + t); for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[j]); }
-        else { const f2_any r = *(const f2_any*)(p + t); v[0] = r[0]; v[1] = r[1]; }
+// workgroup, on the token grid of the tensor.  A tile that holds several segments is walked once for each; what is loaded of
+// the others' tokens stays in its own columns and is not stored.
+template <int TT> __device__ __forceinline__ void load_tokens(float (&v)[TT], const float* p, int64_t t, int64_t tokens) {
+    if (t + TT <= tokens) {
+        if constexpr (TT == 4) {
+            const raw4 r = *(const raw4_f*)(p + t);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[j]);
+        } else if constexpr (TT == 2) { const f2_any r = *(const f2_any*)(p + t); v[0] = r[0]; v[1] = r[1]; }
+        else v[0] = p[t];
         return;
     }
 #pragma unroll
-    for (int j = 0; j < TT; ++j) v[j] = t + j >= lo && t + j < hi ? p[t + j] : 0.f;
+    for (int j = 0; j < TT; ++j) v[j] = t + j < tokens ? p[t + j] : 0.f;
 }
-template <int RT, int TT>
-__global__ __launch_bounds__(64 * kWaves) void lora_cols_kernel(SegTable sg, k82_lora p) {
-    __shared__ Shared<float, RT, TT> sh;
+template <int NW, int RT, int TT>
+__global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lora p) {
+    constexpr int U = 2;
+    __shared__ __align__(16) char lds[most(NW * RT * 1024, NW * RT * TT * 1024)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    raw4* own = (raw4*)lds + wave * RT * 64;
     const int first = sg.start[0];
     const int tile = first / (16 * TT) * (16 * TT) + (int)blockIdx.x * 16 * TT;
     const int64_t t0 = tile + TT * col;
@@ -233,85 +335,121 @@ __global__ __launch_bounds__(64 * kWaves) void lora_cols_kernel(SegTable sg, k82
         bool in[TT];
 #pragma unroll
         for (int t = 0; t < TT; ++t) { tok[t] = t0 + t; in[t] = tok[t] >= lo && tok[t] < hi; }
-        f4 acc[RT][TT];
-        raw4 h[RT][TT];
+        const int blocks = (p.cout + 15) / 16, stride = NW * gridDim.y;
+        int blk = (int)blockIdx.y * NW + wave;
+        float base[4][TT];
+        raw4 fac[RT];
+        const float* b = (const float*)p.b + (int64_t)max(k, 0) * p.cout * p.rank + 4 * (lane & 3);
+        auto fetch = [&](int blk) {
+            const int c0 = 16 * blk;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+            for (int i = 0; i < 4; ++i) {
+                const int c = c0 + 4 * g + i;
+                if (p.base && c < p.cout) load_tokens<TT>(base[i], (const float*)p.base + (int64_t)c * p.ldbase, t0, p.tokens);
+            }
+            if (k >= 0)
 #pragma unroll
-            for (int t = 0; t < TT; ++t) { acc[r][t] = f4{0.f, 0.f, 0.f, 0.f}; h[r][t] = raw4{0u, 0u, 0u, 0u}; }
+                for (int r = 0; r < RT; ++r) fac[r] = grab(b + (int64_t)min(c0 + (lane >> 2), p.cout - 1) * p.rank + 16 * r, p.rank - 16 * r - 4 * (lane & 3));
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) base[i][t] = 0.f;
+        if (blk < blocks) fetch(blk);
+        Second<float, RT> h[TT];
         if (k >= 0) {
+            f4 acc[RT][TT];
             const float* a[RT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) a[r] = (const float*)p.a + ((int64_t)k * p.rank + min(16 * r + col, p.rank - 1)) * p.cin;
-            auto step = [&](int c0, bool whole) {                // 16 channels: 4 g + i in instruction i
-                float fx[4][TT];
-                raw4 fa[RT];
+            for (int r = 0; r < RT; ++r) {
+                a[r] = (const float*)p.a + ((int64_t)k * p.rank + min(16 * r + (lane >> 2), p.rank - 1)) * p.cin + 4 * (lane & 3);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = c0 + 4 * g + i;
-                    if (whole || c < p.cin) load_tokens<TT>(fx[i], (const float*)p.x + (int64_t)c * p.ldx, t0, lo, hi);
-                    else
+                for (int t = 0; t < TT; ++t) acc[r][t] = f4{0.f, 0.f, 0.f, 0.f};
+            }
+            const float* x = (const float*)p.x + (int64_t)4 * g * p.ldx;
+            auto multiply = [&](const raw4 (&fa)[RT], const float (&fx)[4][TT]) {
 #pragma unroll
-                        for (int t = 0; t < TT; ++t) fx[i][t] = 0.f;
-                }
+                for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fa[r]);
+                wave_fence();
+                raw4 ta[RT];
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
-                    fa[r] = whole ? *(const raw4_f*)(a[r] + c0 + 4 * g) : factor4(a[r] + c0 + 4 * g, p.cin - c0 - 4 * g);
+                for (int r = 0; r < RT; ++r) ta[r] = get_tile(own + r * 64);
+                wave_fence();
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int r = 0; r < RT; ++r)
 #pragma unroll
-                        for (int t = 0; t < TT; ++t)
-                            acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(fa[r][i]), fx[i][t], acc[r][t], 0, 0, 0);
+                        for (int t = 0; t < TT; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ta[r][i]), fx[i][t], acc[r][t], 0, 0, 0);
+            };
+            auto steps = [&](int i0, auto n) {                   // 16 channels a step: 4 g + i in instruction i
+                constexpr int n_ = decltype(n)::value;
+                float fx[n_][4][TT];
+                raw4 fa[n_][RT];
+#pragma unroll
+                for (int u = 0; u < n_; ++u) {
+                    const int c0 = 16 * (i0 + u * NW);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) load_tokens<TT>(fx[u][i], x + (int64_t)(c0 + i) * p.ldx, t0, p.tokens);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) fa[u][r] = *(const raw4_f*)(a[r] + c0);
+                }
+#pragma unroll
+                for (int u = 0; u < n_; ++u) multiply(fa[u], fx[u]);
             };
             const int full = p.cin / 16;
             int i = wave;
-            for (; i < full; i += kWaves) step(16 * i, true);
-            if (i == full && p.cin % 16) step(16 * i, false);
-            join<float, RT, TT>(sh, acc, h, p.rank, p.scale[k], blockIdx.y == 0 ? p.h : nullptr, tok, in);
-        } else if (p.h && blockIdx.y == 0) {
+            for (; i + (U - 1) * NW < full; i += U * NW) steps(i, std::integral_constant<int, U>());
+            if (U > 2 && i + NW < full) { steps(i, std::integral_constant<int, 2>()); i += 2 * NW; }
+            if (i < full) { steps(i, std::integral_constant<int, 1>()); i += NW; }
+            if (i == full && p.cin % 16) {                       // one wave: the last channels, zeros behind them
+                const int c0 = 16 * full;
+                raw4 fa[RT];
+                float fx[4][TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
-                if (in[t])
-                    for (int r = 4 * wave + g; r < p.rank; r += 4 * kWaves) p.h[tok[t] * p.rank + r] = 0.f;
-        }
-        const float* b = (const float*)p.b + (int64_t)max(k, 0) * p.cout * p.rank;
-        const int blocks = (p.cout + 15) / 16;
-        for (int blk = (int)blockIdx.y * kWaves + wave; blk < blocks; blk += kWaves * gridDim.y) {
-            const int c0 = 16 * blk;
-            float y[4][TT];
+                for (int r = 0; r < RT; ++r) fa[r] = grab(a[r] + c0, p.cin - c0 - 4 * (lane & 3));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = c0 + 4 * g + i;
-                if (p.base && c < p.cout) load_tokens<TT>(y[i], (const float*)p.base + (int64_t)c * p.ldbase, t0, lo, hi);
-                else
+                for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                    for (int t = 0; t < TT; ++t) y[i][t] = 0.f;
+                    for (int t = 0; t < TT; ++t) fx[i][t] = 0.f;
+                    if (c0 + 4 * g + i < p.cin) load_tokens<TT>(fx[i], x + (int64_t)(c0 + i) * p.ldx, t0, p.tokens);
+                }
+                multiply(fa, fx);
             }
+            join<float, NW, RT, TT>((f4(*)[RT * TT][64])lds, acc, h, p.rank, p.scale[k], blockIdx.y == 0 ? p.h : nullptr, tok, in);
+        } else if (p.h && blockIdx.y == 0) {
+            const int from = max(tile, (int)lo), n = (min(tile + 16 * TT, (int)hi) - from) * p.rank;
+            for (int i = threadIdx.x; i < n; i += 64 * NW) p.h[(int64_t)from * p.rank + i] = 0.f;
+        }
+        for (; blk < blocks; blk += stride) {
             f4 d[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) d[t] = f4{y[0][t], y[1][t], y[2][t], y[3][t]};
+            for (int t = 0; t < TT; ++t) d[t] = f4{base[0][t], base[1][t], base[2][t], base[3][t]};
+            raw4 tb[RT];
             if (k >= 0) {
-                const float* q = b + (int64_t)min(c0 + col, p.cout - 1) * p.rank + 4 * g;
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const raw4 f = factor4(q + 16 * r, p.rank - 16 * r - 4 * g);
+                for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fac[r]);
+                wave_fence();
 #pragma unroll
-                    for (int t = 0; t < TT; ++t) d[t] = product<float>(f, h[r][t], d[t]);
-                }
+                for (int r = 0; r < RT; ++r) tb[r] = get_tile(own + r * 64);
+                wave_fence();
             }
+            if (blk + stride < blocks) fetch(blk + stride);      // the next block is on its way while this one is multiplied
+            if (k >= 0)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) d[t] = h[t].times(tb, d[t]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int c = c0 + 4 * g + i;
-                if (c >= p.cout) continue;
-                float* q = (float*)p.y + (int64_t)c * p.ldy + t0;
+                const int c = 16 * blk + 4 * g + i;
                 float v[TT];
 #pragma unroll
                 for (int t = 0; t < TT; ++t) v[t] = p.act == K82_ACT_GELU_NEW ? op_gelu_new(d[t][i]) : d[t][i];
+                if (c >= p.cout) continue;
+                float* q = (float*)p.y + (int64_t)c * p.ldy + t0;
                 if (in[0] && in[TT - 1]) {
                     if constexpr (TT == 4) *(raw4_f*)q = raw4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-                    else *(f2_any*)q = f2_any{v[0], v[1]};
+                    else if constexpr (TT == 2) *(f2_any*)q = f2_any{v[0], v[1]};
+                    else q[0] = v[0];
                 } else
 #pragma unroll
                     for (int t = 0; t < TT; ++t)
@@ -320,6 +458,8 @@ __global__ __launch_bounds__(64 * kWaves) void lora_cols_kernel(SegTable sg, k82
         }
     }
 }
+
+constexpr int kWaves = 4;                      // of the weight's gradient
 
 // Backward.  dx = dx_base + s_k (dy B_k) A_k is the forward operator with B_k^T and A_k^T for A and B, and the h it keeps is
 // g / s_k = dy B_k.  The transposed factors of the adapters in use are laid out here, side by side in the order of their index.
@@ -482,18 +622,19 @@ int parts(int tiles, int cout) { return std::max(1, std::min((cout + 255) / 256,
 
 template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::Seg>& segs, hipStream_t st) {
     return by_rank(p.rank, [&](auto rt) -> hipError_t {
-        constexpr int RT = decltype(rt)::value, TT = RT == 4 ? 4 : 2;
+        constexpr int RT = decltype(rt)::value, TT = 2, NW = 4;
         if constexpr (std::is_same<T, float>::value)
             if (p.layout == K82_COLS) {
+                constexpr int CT = 2, CW = RT <= 2 ? 8 : 4;
                 for (const SegTable& t : op::tables(segs, 1)) {
-                    const int first = t.start[0], last = first + t.tile0[t.n] - 1, tiles = last / 32 - first / 32 + 1;
-                    OP_TRY(op::run(lora_cols_kernel<RT, 2>, dim3(tiles, parts(tiles, p.cout)), dim3(64 * kWaves), 0, st, t, p));
+                    const int first = t.start[0], last = first + t.tile0[t.n] - 1, tiles = last / (16 * CT) - first / (16 * CT) + 1;
+                    OP_TRY(op::run(lora_cols_kernel<CW, RT, CT>, dim3(tiles, parts(tiles, p.cout)), dim3(64 * CW), 0, st, t, p));
                 }
                 return hipSuccess;
             }
         for (const SegTable& t : op::tables(segs, 16 * TT)) {
             const int tiles = t.tile0[t.n];
-            OP_TRY(op::run(lora_rows_kernel<T, RT, TT>, dim3(tiles, parts(tiles, p.cout)), dim3(64 * kWaves), 0, st, t, p));
+            OP_TRY(op::run(lora_rows_kernel<T, NW, RT, TT>, dim3(tiles, parts(tiles, p.cout)), dim3(64 * NW), 0, st, t, p));
         }
         return hipSuccess;
     });
