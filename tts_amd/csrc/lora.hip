@@ -39,7 +39,16 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-template <class T> __device__ __forceinline__ raw4 grab(const T* p, int n) { return n > 0 ? load_part(p, n) : raw4{0u, 0u, 0u, 0u}; }
+// 16 bytes at a uniform base and a lane's own 32-bit offset (one register a lane for an address; rows are at most 2^25 long)
+__device__ __forceinline__ raw4 load16(const char* base, uint32_t at) { return *(const raw4_any*)(base + at); }
+// The same at a place that may lie in part (EVEN: as a whole) behind the row: n elements from there on are in the row, `back`
+// bytes before it there is some.
+template <class T, bool EVEN> __device__ __forceinline__ raw4 grab(const char* base, uint32_t at, int n, uint32_t back) {
+    if constexpr (EVEN) {
+        const raw4 r = load16(base, n > 0 ? at : at - back), zero = {0u, 0u, 0u, 0u};
+        return n > 0 ? r : zero;
+    } else return n > 0 ? load_part((const T*)(base + at), n) : raw4{0u, 0u, 0u, 0u};
+}
 __device__ __forceinline__ void put_tile(raw4* tile, raw4 v) {
     const int lane = threadIdx.x & 63;
     tile[(lane & ~3) + ((lane & 3) ^ (lane >> 4))] = v;
@@ -128,7 +137,7 @@ __device__ __forceinline__ void join(f4 (*part)[RT * TT][64], f4 (&acc)[RT][TT],
         for (int r = 0; r < RT; ++r) {
             const int i = r * TT + t;
             f4 v = part[0][i][lane];
-#pragma unroll
+#pragma unroll 3
             for (int w = 1; w < NW; ++w) v += part[w][i][lane];
             const int r0 = rank_of<T, RT>(r, 4 * g);
 #pragma unroll
@@ -154,9 +163,10 @@ constexpr int kPad = 4;                        // floats behind a row of the res
 // NW-th 64 bytes of a row, so together they read 64 NW contiguous bytes) and the output channels of the second, 128 bytes of a
 // row a wave at a time.  The results cross LDS once more, so that base and y are read and written in whole lines.
 // blockIdx.y splits the output channels where there are few tokens; each part then computes h for itself, from cache.
-template <class T, int NW, int RT, int TT>
+// EVEN: cin, cout and rank are multiples of a lane's 16 bytes, no place lies in part behind a row.
+template <class T, int NW, int RT, int TT, bool EVEN>
 __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lora p) {
-    constexpr int V = Vec<T>::N, K = 4 * V, U = RT + TT > 4 ? 2 : 4;             // U: steps whose loads are in flight together
+    constexpr int V = Vec<T>::N, K = 4 * V, S = sizeof(T), U = RT + TT > 4 ? 2 : 4;          // U: steps whose loads are in flight together
     constexpr int CH = 8 * V, MT = CH / 16, CK = Second<T, RT>::CHUNKS;          // channels, row tiles of B, chunks of a row of B
     constexpr int kTiles = most(RT + TT, MT * CK), kRow = CH + kPad;
     constexpr int kOwn = most(kTiles * 1024, MT * CK * 1024 + 16 * kRow * 4);    // a wave's own bytes
@@ -166,25 +176,29 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
     if (k < 0 && p.act == K82_ACT_NONE && p.base == p.y && !p.h) return;
     raw4* own = (raw4*)(lds + wave * kOwn);
     float* result = (float*)(own + MT * CK * 64);
-    const int row0 = ((int)blockIdx.x - sg.tile0[s]) * 16 * TT, last = sg.len[s] - 1;
-    const int64_t t0 = sg.start[s];
-    // Second product: this lane's 16 bytes of rows (lane / 8) + 8 i of the tokens
-    const int blocks = (p.cout + CH - 1) / CH, stride = NW * gridDim.y;
+    const int row0 = ((int)blockIdx.x - sg.tile0[s]) * 16 * TT, last = sg.len[s] - 1 - row0;
+    const int64_t t0 = sg.start[s] + row0;
+    // Second product: this lane's 16 bytes of the tokens (lane / 8) + 8 i
+    const int blocks = (p.cout + CH - 1) / CH, stride = NW * gridDim.y, c8 = V * (lane & 7), c4 = V * (lane & 3);
+    const char* basep = (const char*)p.base + t0 * p.ldbase * S;
+    char* yp = (char*)p.y + t0 * p.ldy * S;
+    const char* bp = (const char*)p.b + (int64_t)max(k, 0) * p.cout * p.rank * S;
     int blk = (int)blockIdx.y * NW + wave;
     raw4 base[2 * TT], fac[MT * CK];
-    const T* b = (const T*)p.b + (int64_t)max(k, 0) * p.cout * p.rank;
     auto fetch = [&](int blk) {
-        const int c = blk * CH + V * (lane & 7);
+        const int n = p.cout - blk * CH;
         if (p.base) {
 #pragma unroll
-            for (int i = 0; i < 2 * TT; ++i) base[i] = grab((const T*)p.base + (t0 + min(row0 + 8 * i + (lane >> 3), last)) * p.ldbase + c, p.cout - c);
+            for (int i = 0; i < 2 * TT; ++i)
+                base[i] = grab<T, EVEN>(basep + (int64_t)blk * CH * S, (min(8 * i + (lane >> 3), last) * (uint32_t)p.ldbase + c8) * S, n - c8, c8 * S);
         }
         if (k >= 0) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const T* q = b + (int64_t)min(blk * CH + 16 * m + (lane >> 2), p.cout - 1) * p.rank + V * (lane & 3);
+                const uint32_t at = (min(16 * m + (lane >> 2), n - 1) * (uint32_t)p.rank + c4) * S;
 #pragma unroll
-                for (int c = 0; c < CK; ++c) fac[m * CK + c] = grab(q + c * K, p.rank - c * K - V * (lane & 3));
+                for (int c = 0; c < CK; ++c)
+                    fac[m * CK + c] = grab<T, EVEN>(bp + (int64_t)blk * CH * p.rank * S, at + c * K * S, p.rank - c * K - c4, (c * K + c4) * S);
             }
         }
     };
@@ -194,11 +208,12 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
     Second<T, RT> h[TT];
     if (k >= 0) {
         f4 acc[RT][TT];
-        const T *a[RT], *x[TT];
+        const char *ap = (const char*)p.a + (int64_t)k * p.rank * p.cin * S, *xp = (const char*)p.x + t0 * p.ldx * S;
+        uint32_t ao[RT], xo[TT];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) a[r] = (const T*)p.a + ((int64_t)k * p.rank + min(rank_of<T, RT>(r, lane >> 2), p.rank - 1)) * p.cin + V * (lane & 3);
+        for (int r = 0; r < RT; ++r) ao[r] = (min(rank_of<T, RT>(r, lane >> 2), p.rank - 1) * (uint32_t)p.cin + c4) * S;
 #pragma unroll
-        for (int t = 0; t < TT; ++t) x[t] = (const T*)p.x + (t0 + min(row0 + 16 * t + (lane >> 2), last)) * p.ldx + V * (lane & 3);
+        for (int t = 0; t < TT; ++t) xo[t] = (min(16 * t + (lane >> 2), last) * (uint32_t)p.ldx + c4) * S;
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -226,11 +241,11 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
             raw4 fa[n_][RT], fx[n_][TT];
 #pragma unroll
             for (int i = 0; i < n_; ++i) {
-                const int at = (i0 + i * NW) * K;
+                const int at = (i0 + i * NW) * K * S;
 #pragma unroll
-                for (int t = 0; t < TT; ++t) fx[i][t] = *(const raw4_any*)(x[t] + at);
+                for (int t = 0; t < TT; ++t) fx[i][t] = load16(xp + at, xo[t]);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) fa[i][r] = *(const raw4_any*)(a[r] + at);
+                for (int r = 0; r < RT; ++r) fa[i][r] = load16(ap + at, ao[r]);
             }
 #pragma unroll
             for (int i = 0; i < n_; ++i) multiply(fa[i], fx[i]);
@@ -240,22 +255,22 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
         if (U > 2 && i + NW < full) { steps(i, std::integral_constant<int, 2>()); i += 2 * NW; }
         if (i < full) { steps(i, std::integral_constant<int, 1>()); i += NW; }
         if (i == full && p.cin % K) {                            // one wave: the end of the row, zeros behind it
-            const int at = full * K, n = p.cin - at - V * (lane & 3);
+            const int at = full * K, n = p.cin - at - c4;
             raw4 fa[RT], fx[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) fx[t] = grab(x[t] + at, n);
+            for (int t = 0; t < TT; ++t) fx[t] = grab<T, EVEN>(xp + at * S, xo[t], n, c4 * S);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) fa[r] = grab(a[r] + at, n);
+            for (int r = 0; r < RT; ++r) fa[r] = grab<T, EVEN>(ap + at * S, ao[r], n, c4 * S);
             multiply(fa, fx);
         }
         int64_t tok[TT];
         bool in[TT];
 #pragma unroll
-        for (int t = 0; t < TT; ++t) { tok[t] = t0 + row0 + 16 * t + col; in[t] = row0 + 16 * t + col <= last; }
+        for (int t = 0; t < TT; ++t) { tok[t] = t0 + 16 * t + col; in[t] = 16 * t + col <= last; }
         join<T, NW, RT, TT>((f4(*)[RT * TT][64])lds, acc, h, p.rank, p.scale[k], blockIdx.y == 0 ? p.h : nullptr, tok, in);
     } else if (p.h && blockIdx.y == 0) {
-        const int n = min(16 * TT, last + 1 - row0) * p.rank;
-        for (int i = threadIdx.x; i < n; i += 64 * NW) p.h[(t0 + row0) * p.rank + i] = 0.f;
+        const int n = min(16 * TT, last + 1) * p.rank;
+        for (int i = threadIdx.x; i < n; i += 64 * NW) p.h[t0 * p.rank + i] = 0.f;
     }
     for (; blk < blocks; blk += stride) {
         raw4 now[2 * TT], tile[MT][CK];
@@ -271,7 +286,8 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
                 for (int c = 0; c < CK; ++c) tile[m][c] = get_factor<T, RT>(own + (m * CK + c) * 64);
         }
         if (blk + stride < blocks) fetch(blk + stride);          // the next block is on its way while this one is multiplied
-        const int c = blk * CH + V * (lane & 7), n = p.cout - c;
+        const int n = p.cout - blk * CH - c8;
+        char* yb = yp + (int64_t)blk * CH * S;
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             if (k >= 0) {
@@ -286,15 +302,19 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
                 if (k >= 0) {
 #pragma unroll
                     for (int j = 0; j < V; j += 4) {
-                        const f4 d = *(const f4*)(result + (8 * i + (lane >> 3)) * kRow + V * (lane & 7) + j);
+                        const f4 d = *(const f4*)(result + (8 * i + (lane >> 3)) * kRow + c8 + j);
                         f[j] += d[0]; f[j + 1] += d[1]; f[j + 2] += d[2]; f[j + 3] += d[3];
                     }
                 }
                 if (p.act == K82_ACT_GELU_NEW)
 #pragma unroll
                     for (int j = 0; j < V; ++j) f[j] = op_gelu_new(f[j]);
-                const int row = row0 + 16 * t + 8 * i + (lane >> 3);
-                if (row <= last && n > 0) store_part((T*)p.y + (t0 + row) * p.ldy + c, f, n);
+                const int row = 16 * t + 8 * i + (lane >> 3);
+                if (row <= last && n > 0) {
+                    T* q = (T*)(yb + (row * (uint32_t)p.ldy + c8) * S);
+                    if constexpr (EVEN) *(raw4_any*)q = Vec<T>::pack(f);
+                    else store_part(q, f, n);
+                }
             }
             wave_fence();
         }
@@ -304,52 +324,46 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
 // Channel-first: the same products, TT consecutive tokens a lane (tile t of a lane's tokens is TT col + t), 16 TT tokens a
 // workgroup, on the token grid of the tensor.  A tile that holds several segments is walked once for each; what is loaded of
 // the others' tokens stays in its own columns and is not stored.
-template <int TT> __device__ __forceinline__ void load_tokens(float (&v)[TT], const float* p, int64_t t, int64_t tokens) {
-    if (t + TT <= tokens) {
-        if constexpr (TT == 4) {
-            const raw4 r = *(const raw4_f*)(p + t);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r[j]);
-        } else if constexpr (TT == 2) { const f2_any r = *(const f2_any*)(p + t); v[0] = r[0]; v[1] = r[1]; }
-        else v[0] = p[t];
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < TT; ++j) v[j] = t + j < tokens ? p[t + j] : 0.f;
+// The last tile reads at the tensor's end (t = its last pair, or token) and takes what is left: `second` where that pair is one
+// token ahead of the lane's.  at: bytes of the row
+template <int TT> __device__ __forceinline__ void load_tokens(float (&v)[TT], const char* base, uint32_t at, bool second) {
+    if constexpr (TT == 2) {
+        const f2_any r = *(const f2_any*)(base + at);
+        v[0] = second ? r[1] : r[0];
+        v[1] = r[1];
+    } else v[0] = *(const float*)(base + at);
 }
-template <int NW, int RT, int TT>
+template <int NW, int RT, int TT, bool EVEN>
 __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lora p) {
     constexpr int U = 2;
     __shared__ __align__(16) char lds[most(NW * RT * 1024, NW * RT * TT * 1024)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     raw4* own = (raw4*)lds + wave * RT * 64;
-    const int first = sg.start[0];
-    const int tile = first / (16 * TT) * (16 * TT) + (int)blockIdx.x * 16 * TT;
-    const int64_t t0 = tile + TT * col;
+    const int first = sg.start[0], tokens = (int)p.tokens, c4 = 4 * (lane & 3);
+    const int tile = first / (16 * TT) * (16 * TT) + (int)blockIdx.x * 16 * TT, t0 = tile + TT * col;
+    const uint32_t tb = 4 * min(t0, tokens - TT);
+    const bool second = t0 == tokens - 1;
     int s = place(sg.tile0, max(tile, first) - first);
     for (; s < sg.n && sg.start[s] < tile + 16 * TT; ++s) {
-        const int k = sg.index[s];
-        const int64_t lo = sg.start[s], hi = (int64_t)sg.start[s] + sg.len[s];
+        const int k = sg.index[s], lo = sg.start[s], hi = lo + sg.len[s];
         if (k < 0 && p.act == K82_ACT_NONE && p.base == p.y && !p.h) continue;
-        int64_t tok[TT];
-        bool in[TT];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) { tok[t] = t0 + t; in[t] = tok[t] >= lo && tok[t] < hi; }
         const int blocks = (p.cout + 15) / 16, stride = NW * gridDim.y;
         int blk = (int)blockIdx.y * NW + wave;
         float base[4][TT];
         raw4 fac[RT];
-        const float* b = (const float*)p.b + (int64_t)max(k, 0) * p.cout * p.rank + 4 * (lane & 3);
+        const char* bp = (const char*)p.b + (int64_t)max(k, 0) * p.cout * p.rank * 4;
         auto fetch = [&](int blk) {
-            const int c0 = 16 * blk;
+            const int n = p.cout - 16 * blk;
+            if (p.base) {
+                const char* q = (const char*)p.base + (int64_t)16 * blk * p.ldbase * 4;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = c0 + 4 * g + i;
-                if (p.base && c < p.cout) load_tokens<TT>(base[i], (const float*)p.base + (int64_t)c * p.ldbase, t0, p.tokens);
+                for (int i = 0; i < 4; ++i) load_tokens<TT>(base[i], q, min(4 * g + i, n - 1) * (uint32_t)p.ldbase * 4 + tb, second);
             }
-            if (k >= 0)
+            if (k >= 0) {
+                const uint32_t at = (min(lane >> 2, n - 1) * (uint32_t)p.rank + c4) * 4;
 #pragma unroll
-                for (int r = 0; r < RT; ++r) fac[r] = grab(b + (int64_t)min(c0 + (lane >> 2), p.cout - 1) * p.rank + 16 * r, p.rank - 16 * r - 4 * (lane & 3));
+                for (int r = 0; r < RT; ++r) fac[r] = grab<float, EVEN>(bp + (int64_t)16 * blk * p.rank * 4, at + 64 * r, p.rank - 16 * r - c4, (16 * r + c4) * 4);
+            }
         };
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -359,14 +373,14 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
         Second<float, RT> h[TT];
         if (k >= 0) {
             f4 acc[RT][TT];
-            const float* a[RT];
+            uint32_t ao[RT];
+            const char* ap = (const char*)p.a + (int64_t)k * p.rank * p.cin * 4;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                a[r] = (const float*)p.a + ((int64_t)k * p.rank + min(16 * r + (lane >> 2), p.rank - 1)) * p.cin + 4 * (lane & 3);
+                ao[r] = (min(16 * r + (lane >> 2), p.rank - 1) * (uint32_t)p.cin + c4) * 4;
 #pragma unroll
                 for (int t = 0; t < TT; ++t) acc[r][t] = f4{0.f, 0.f, 0.f, 0.f};
             }
-            const float* x = (const float*)p.x + (int64_t)4 * g * p.ldx;
             auto multiply = [&](const raw4 (&fa)[RT], const float (&fx)[4][TT]) {
 #pragma unroll
                 for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fa[r]);
@@ -389,10 +403,11 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
 #pragma unroll
                 for (int u = 0; u < n_; ++u) {
                     const int c0 = 16 * (i0 + u * NW);
+                    const char* q = (const char*)p.x + (int64_t)c0 * p.ldx * 4;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) load_tokens<TT>(fx[u][i], x + (int64_t)(c0 + i) * p.ldx, t0, p.tokens);
+                    for (int i = 0; i < 4; ++i) load_tokens<TT>(fx[u][i], q, (4 * g + i) * (uint32_t)p.ldx * 4 + tb, second);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) fa[u][r] = *(const raw4_f*)(a[r] + c0);
+                    for (int r = 0; r < RT; ++r) fa[u][r] = load16(ap + 4 * c0, ao[r]);
                 }
 #pragma unroll
                 for (int u = 0; u < n_; ++u) multiply(fa[u], fx[u]);
@@ -400,25 +415,29 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
             const int full = p.cin / 16;
             int i = wave;
             for (; i + (U - 1) * NW < full; i += U * NW) steps(i, std::integral_constant<int, U>());
-            if (U > 2 && i + NW < full) { steps(i, std::integral_constant<int, 2>()); i += 2 * NW; }
             if (i < full) { steps(i, std::integral_constant<int, 1>()); i += NW; }
             if (i == full && p.cin % 16) {                       // one wave: the last channels, zeros behind them
-                const int c0 = 16 * full;
+                const int c0 = 16 * full, n = p.cin - c0;
+                const char* q = (const char*)p.x + (int64_t)c0 * p.ldx * 4;
                 raw4 fa[RT];
                 float fx[4][TT];
 #pragma unroll
-                for (int r = 0; r < RT; ++r) fa[r] = grab(a[r] + c0, p.cin - c0 - 4 * (lane & 3));
+                for (int r = 0; r < RT; ++r) fa[r] = grab<float, EVEN>(ap + 4 * c0, ao[r], n - c4, 4 * c4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    load_tokens<TT>(fx[i], q, min(4 * g + i, n - 1) * (uint32_t)p.ldx * 4 + tb, second);
 #pragma unroll
-                    for (int t = 0; t < TT; ++t) fx[i][t] = 0.f;
-                    if (c0 + 4 * g + i < p.cin) load_tokens<TT>(fx[i], x + (int64_t)(c0 + i) * p.ldx, t0, p.tokens);
+                    for (int t = 0; t < TT; ++t) fx[i][t] = 4 * g + i < n ? fx[i][t] : 0.f;
                 }
                 multiply(fa, fx);
             }
+            int64_t tok[TT];
+            bool in[TT];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) { tok[t] = t0 + t; in[t] = t0 + t >= lo && t0 + t < hi; }
             join<float, NW, RT, TT>((f4(*)[RT * TT][64])lds, acc, h, p.rank, p.scale[k], blockIdx.y == 0 ? p.h : nullptr, tok, in);
         } else if (p.h && blockIdx.y == 0) {
-            const int from = max(tile, (int)lo), n = (min(tile + 16 * TT, (int)hi) - from) * p.rank;
+            const int from = max(tile, lo), n = (min(tile + 16 * TT, hi) - from) * p.rank;
             for (int i = threadIdx.x; i < n; i += 64 * NW) p.h[(int64_t)from * p.rank + i] = 0.f;
         }
         for (; blk < blocks; blk += stride) {
@@ -438,22 +457,22 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
             if (k >= 0)
 #pragma unroll
                 for (int t = 0; t < TT; ++t) d[t] = h[t].times(tb, d[t]);
+            char* yb = (char*)p.y + (int64_t)16 * blk * p.ldy * 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int c = 16 * blk + 4 * g + i;
+                const int c = 4 * g + i;
                 float v[TT];
 #pragma unroll
                 for (int t = 0; t < TT; ++t) v[t] = p.act == K82_ACT_GELU_NEW ? op_gelu_new(d[t][i]) : d[t][i];
-                if (c >= p.cout) continue;
-                float* q = (float*)p.y + (int64_t)c * p.ldy + t0;
-                if (in[0] && in[TT - 1]) {
-                    if constexpr (TT == 4) *(raw4_f*)q = raw4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-                    else if constexpr (TT == 2) *(f2_any*)q = f2_any{v[0], v[1]};
+                if (16 * blk + c >= p.cout) continue;
+                float* q = (float*)(yb + (c * (uint32_t)p.ldy + t0) * 4);
+                if (t0 >= lo && t0 + TT <= hi) {
+                    if constexpr (TT == 2) *(f2_any*)q = f2_any{v[0], v[1]};
                     else q[0] = v[0];
                 } else
 #pragma unroll
                     for (int t = 0; t < TT; ++t)
-                        if (in[t]) q[t] = v[t];
+                        if (t0 + t >= lo && t0 + t < hi) q[t] = v[t];
             }
         }
     }
@@ -617,24 +636,34 @@ template <class F> hipError_t by_rank(int rank, F&& f) {
     if (rank <= 64) return f(std::integral_constant<int, 4>());
     return f(std::integral_constant<int, 8>());
 }
-// parts of the output channels: until there are two workgroups a CU, at least 64 channels a wave
-int parts(int tiles, int cout) { return std::max(1, std::min((cout + 255) / 256, 512 / std::max(1, tiles))); }
+// Parts of the output channels: until there are two workgroups a CU, `wide` channels (a block for each wave) at least.  More
+// parts cost more first products than their balance gains: 16411 x 768 f32 channel-first 48 us, with up to 1100 workgroups 56.
+int parts(int tiles, int cout, int wide) { return std::max(1, std::min((cout + wide - 1) / wide, 512 / std::max(1, tiles))); }
 
 template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::Seg>& segs, hipStream_t st) {
     return by_rank(p.rank, [&](auto rt) -> hipError_t {
-        constexpr int RT = decltype(rt)::value, TT = 2, NW = 4;
+        constexpr int RT = decltype(rt)::value, V = Vec<T>::N;
+        const bool even = p.cin % V == 0 && p.cout % V == 0 && p.rank % V == 0;
         if constexpr (std::is_same<T, float>::value)
             if (p.layout == K82_COLS) {
-                constexpr int CT = 2, CW = RT <= 2 ? 8 : 4;
-                for (const SegTable& t : op::tables(segs, 1)) {
-                    const int first = t.start[0], last = first + t.tile0[t.n] - 1, tiles = last / (16 * CT) - first / (16 * CT) + 1;
-                    OP_TRY(op::run(lora_cols_kernel<CW, RT, CT>, dim3(tiles, parts(tiles, p.cout)), dim3(64 * CW), 0, st, t, p));
-                }
-                return hipSuccess;
+                constexpr int NW = RT <= 2 ? 8 : 4;
+                auto go = [&](auto tt) -> hipError_t {
+                    constexpr int TT = decltype(tt)::value;
+                    for (const SegTable& t : op::tables(segs, 1)) {
+                        const int first = t.start[0], last = first + t.tile0[t.n] - 1, tiles = last / (16 * TT) - first / (16 * TT) + 1;
+                        OP_TRY(op::run(even ? lora_cols_kernel<NW, RT, TT, true> : lora_cols_kernel<NW, RT, TT, false>,
+                                       dim3(tiles, parts(tiles, p.cout, 16 * NW)), dim3(64 * NW), 0, st, t, p));
+                    }
+                    return hipSuccess;
+                };
+                // pairs of tokens a lane (128 bytes of a channel a tile), where there is a pair
+                return p.tokens >= 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
             }
+        constexpr int TT = 2, NW = 4;
         for (const SegTable& t : op::tables(segs, 16 * TT)) {
             const int tiles = t.tile0[t.n];
-            OP_TRY(op::run(lora_rows_kernel<T, NW, RT, TT>, dim3(tiles, parts(tiles, p.cout)), dim3(64 * NW), 0, st, t, p));
+            OP_TRY(op::run(even ? lora_rows_kernel<T, NW, RT, TT, true> : lora_rows_kernel<T, NW, RT, TT, false>,
+                           dim3(tiles, parts(tiles, p.cout, 8 * NW * V)), dim3(64 * NW), 0, st, t, p));
         }
         return hipSuccess;
     });
