@@ -120,6 +120,33 @@ int k82_durations(k82_handle* h, const int64_t* ids, const int32_t* lens, int B,
                   const float* ref_s, const float* speed, const int32_t* forced_dur,
                   int32_t* pred_dur, int64_t* n_frames, void* stream);
 
+/* Adapters of tuned voices: low-rank factors beside the Linears of the (layer-shared) ALBERT encoder and / or gains and offsets
+ * in the place of its two layer norms.  Replaces the handle's adapters (n = 0: none); host f32, copied before the call
+ * returns.  A fork (k82_fork) inherits what its parent holds; while forks live, and on a fork, the call is refused
+ * (K82_ESTATE), since they read the same memory.  No counterpart in the reference, whose voices are style vectors only. */
+#define K82_ADAPTER_QUERY 0
+#define K82_ADAPTER_KEY 1
+#define K82_ADAPTER_VALUE 2
+#define K82_ADAPTER_DENSE 3       /* attention output */
+#define K82_ADAPTER_FFN 4
+#define K82_ADAPTER_FFN_OUTPUT 5
+#define K82_ADAPTER_PARTS 6
+typedef struct k82_adapter {
+    int32_t rank;                              /* 1..128 (0 if no part has factors) */
+    float scale;                               /* of every part: y += scale * B (A x) */
+    const float* a[K82_ADAPTER_PARTS];         /* f32[rank][in features], NULL: the part has no factors */
+    const float* b[K82_ADAPTER_PARTS];         /* f32[out features][rank] */
+    const float* gain[2];                      /* f32[768] for attention.LayerNorm, full_layer_layer_norm; NULL: the model's */
+    const float* offset[2];                    /* with gain */
+} k82_adapter;
+int k82_set_adapters(k82_handle* h, const k82_adapter* adapters, int32_t n);
+
+/* k82_durations with an adapter for each sentence: adapter[b] in [-1, n), host i32[B]; -1 (and NULL for all) is the model as
+ * it is.  A sentence gives the same bits whatever the adapters of the others in its batch. */
+int k82_durations_adapted(k82_handle* h, const int64_t* ids, const int32_t* lens, int B, int Tmax, const float* ref_s,
+                          const float* speed, const int32_t* forced_dur, const int32_t* adapter, int32_t* pred_dur,
+                          int64_t* n_frames, void* stream);
+
 /* Phase 2 (frame rate): length regulation, F0/N predictor, text encoder, decoder, iSTFTNet
  * generator for the batch of the preceding k82_durations call.
  *   audio     f32[capacity] host or device out; sentence b occupies

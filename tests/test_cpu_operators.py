@@ -185,3 +185,99 @@ def test_layouts_of_single_tokens_and_channels_are_taken_either_way():
     assert Operators._layout(x=torch.zeros(5, 9)[:, 1:], base=None) == (0, [9, 0])
     assert Operators._layout(x=torch.zeros(9, 32).t()[:5]) == (1, [32])
     assert Operators._layout(x=torch.zeros(7, 3)[:, :1]) == (0, [3])
+
+
+# ---------------------------------------------------------------------------------------------- adapters of voices
+def small_adapter(rank=4, parts=("query", "ffn"), norms=("full_norm",), seed=0, scale=0.5):
+    from tts_amd import Adapter
+    from tts_amd.adapters import part_shape
+    r = np.random.default_rng(seed)
+    f = {p: (r.standard_normal((rank, part_shape(p)[0])), r.standard_normal((part_shape(p)[1], rank))) for p in parts}
+    return Adapter(f, scale, {m: (r.standard_normal(768), r.standard_normal(768)) for m in norms})
+
+
+def test_adapter_files_come_back_as_they_went(tmp_path):
+    from tts_amd import Adapter
+    a = small_adapter()
+    a.save(tmp_path / "voice.npz")
+    b = Adapter.load(tmp_path / "voice.npz")
+    assert (b.rank, b.scale, set(b.factors), set(b.norms)) == (4, 0.5, {"query", "ffn"}, {"full_norm"})
+    for part in a.factors:
+        for x, y in zip(a.factors[part], b.factors[part]):
+            assert x.dtype == np.float32 and np.array_equal(x, y)
+    s = b.c_struct()
+    assert s.rank == 4 and s.a[0] and s.b[0] and not s.a[1] and s.a[4] and s.gain[1] and not s.gain[0]
+    np.savez(tmp_path / "odd.npz", **{"query.a": a.factors["query"][0], "query.b": a.factors["query"][1], "else": np.zeros(3)})
+    with pytest.raises(ValueError, match="unexpected arrays"):
+        Adapter.load(tmp_path / "odd.npz")
+    np.savez(tmp_path / "half.npz", **{"query.a": a.factors["query"][0]})
+    with pytest.raises(KeyError):
+        Adapter.load(tmp_path / "half.npz")
+
+
+def test_adapters_that_do_not_fit_are_refused():
+    from tts_amd import Adapter
+    z = np.zeros
+    for factors, norms, word in (
+            ({"nose": (z((2, 768)), z((768, 2)))}, {}, "unknown part"), ({"ffn": (z((2, 768)), z((768, 2)))}, {}, "ffn needs"),
+            ({"query": (z((129, 768)), z((768, 129)))}, {}, "rank 1 to 128"), ({"query": (z((2, 768)), z((768, 3)))}, {}, "query needs"),
+            ({"query": (z((0, 768)), z((768, 0)))}, {}, "rank 1 to 128"),
+            ({"query": (z((2, 768)), z((768, 2))), "key": (z((3, 768)), z((768, 3)))}, {}, "one rank"),
+            ({}, {"full_norm": (z(768), z(767))}, "gain and an offset"), ({}, {"norm": (z(768), z(768))}, "unknown norm")):
+        with pytest.raises(ValueError, match=word):
+            Adapter(factors, 1.0, norms)
+    with pytest.raises(ValueError, match="finite"):
+        Adapter({}, float("inf"))
+
+
+def test_names_of_adapters_are_resolved_for_the_batch():
+    from tts_amd import Engine
+    e = object.__new__(Engine)
+    e.h = C.c_void_p()
+    e._adapters = {"x": 0, "y": 1}
+    assert e._adapter_indices(None, 3) is None
+    assert e._adapter_indices(["y", None, "x"], 3).tolist() == [1, -1, 0]
+    with pytest.raises(ValueError, match="2 sentences, the batch has 3"):
+        e._adapter_indices(["x", "y"], 3)
+    with pytest.raises(KeyError, match="'z' not found"):
+        e._adapter_indices(["z"], 1)
+    with pytest.raises(TypeError, match="not a tts_amd.Adapter"):
+        e.set_adapters({"x": 3})
+
+
+def test_the_scheduler_hands_adapters_to_their_sentences():
+    from tts_amd.scheduler import BatchSynthesizer
+    seen = {}
+
+    class Fake:
+        device = 0
+
+        def pack(self, id_lists):
+            lens = np.array([len(x) + 2 for x in id_lists], np.int32)
+            self.now = [tuple(x) for x in id_lists]
+            return np.zeros((len(id_lists), lens.max()), np.int64), lens
+
+        def session(self):
+            import contextlib
+            return contextlib.nullcontext(self)
+
+        def durations(self, ids, lens, refs, speed=None, **more):
+            for k, x in enumerate(self.now):
+                seen.setdefault(x, []).append(more["adapters"][k] if more else "none given")
+            self.n = np.array([1 if x[0] != 9 else 50 for x in self.now], np.int64)      # ragged: the batch is split and run again
+            return np.ones((len(lens), lens.max()), np.int32), self.n
+
+        def decode(self, seeds=None):
+            off = np.concatenate([[0], np.cumsum(600 * self.n)])
+            return np.zeros(off[-1], np.float32), off
+
+    ids = [[1], [2, 2], [9, 9, 9], [4, 4]]
+    names = ["a", None, "b", "a"]
+    s = BatchSynthesizer(Fake(), frame_pad_limit=1.5)
+    assert len(s.synthesize(ids, [np.zeros(256, np.float32)] * 4, adapters=names)) == 4
+    assert s.stats["rebucketed"] >= 1
+    for x, n in zip(ids, names):
+        assert set(seen[tuple(x)]) == {n}
+    seen.clear()
+    s.synthesize(ids, [np.zeros(256, np.float32)] * 4)
+    assert {v for w in seen.values() for v in w} == {"none given"}

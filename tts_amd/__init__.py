@@ -4,7 +4,7 @@ Front doors: ``Kokoro`` (the reference's real boundary, speech7.py:82,127), ``KP
 ``KModel`` (north_star API).  Everything computes in ``libk82.so`` (tts_amd/csrc, C-ABI in
 include/k82.h); nothing is initialised at import time.
 """
-__all__ = ["Kokoro", "KPipeline", "KModel", "Engine", "Operators", "Segments", "TTSEngine", "EpubBook", "SAMPLE_RATE"]
+__all__ = ["Kokoro", "KPipeline", "KModel", "Engine", "Operators", "Segments", "Adapter", "TTSEngine", "EpubBook", "SAMPLE_RATE"]
 SAMPLE_RATE = 24000
 
 
@@ -24,4 +24,7 @@ def __getattr__(name):
     if name in ("Operators", "Segments"):
         from . import operators
         return getattr(operators, name)
+    if name == "Adapter":
+        from .adapters import Adapter
+        return Adapter
     raise AttributeError(name)

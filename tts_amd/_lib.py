@@ -14,7 +14,7 @@ K82_OK, K82_ENOSPC = 0, -28
 EXPORTS = (
     "k82_create", "k82_fork", "k82_destroy", "k82_last_error", "k82_set_tensor", "k82_finalize", "k82_durations",
     "k82_decode", "k82_synthesize", "k82_reserve", "k82_pcm16", "k82_pcm16_static", "k82_set_precision", "k82_prof_enable", "k82_prof_read", "k82_debug_enable",
-    "k82_debug_info", "k82_debug_copy", "k82_debug_force", "k82_op_conv1d", "k82_op_lora",
+    "k82_debug_info", "k82_debug_copy", "k82_debug_force", "k82_op_conv1d", "k82_set_adapters", "k82_durations_adapted", "k82_op_lora",
     "k82_op_lora_check", "k82_op_lora_grad", "k82_op_lora_grad_workspace", "k82_op_layernorm", "k82_op_layernorm_check",
     "k82_op_layernorm_grad", "k82_op_layernorm_grad_workspace",
 )
@@ -48,6 +48,11 @@ K82LayernormGrad = _struct("K82LayernormGrad", (_i32, "dtype c gains"), (_i64, "
                            (_vp, "res"), (_i64, "ldres"), (_vp, "dy"), (_i64, "lddy"), (_vp, "dx"), (_i64, "lddx"),
                            (_vp, "gain mean rstd dgain doffset"))
 
+
+class K82Adapter(C.Structure):
+    _fields_ = [("rank", _i32), ("scale", _f32), ("a", _vp * 6), ("b", _vp * 6), ("gain", _vp * 2), ("offset", _vp * 2)]
+
+
 _lib = None
 
 
@@ -77,6 +82,8 @@ def load():
     lib.k82_set_tensor.argtypes = [vp, C.c_char_p, f32p, C.POINTER(i64), i32]
     lib.k82_finalize.argtypes = [vp]
     lib.k82_durations.argtypes = [vp, vp, vp, i32, i32, vp, vp, vp, vp, vp, vp]
+    lib.k82_durations_adapted.argtypes = [vp, vp, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp]
+    lib.k82_set_adapters.argtypes = [vp, vp, C.c_int32]
     lib.k82_decode.argtypes = [vp, C.POINTER(K82Noise), vp, i64, vp, vp]
     lib.k82_synthesize.argtypes = [vp, vp, vp, i32, i32, vp, vp, C.POINTER(K82Noise), vp, vp, i64, vp, vp]
     lib.k82_set_precision.argtypes = [vp, C.c_int]

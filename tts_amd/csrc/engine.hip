@@ -173,6 +173,14 @@ struct ResBlock1W {
     float *a1[3], *ia1[3], *a2[3], *ia2[3]; int C = 0, k = 0;
 };
 struct LNW { float* w; float* b; };
+// Adapters of tuned voices (k82_set_adapters), side by side: factors [n][rank][cin] / [n][cout][rank] of every ALBERT Linear at
+// the largest rank (zeros behind an adapter's own), norm rows [n][768].
+struct Adapters {
+    int n = 0, rank = 0;
+    char* mem = nullptr;                       // one allocation, owned by the handle that made it
+    float *a[K82_ADAPTER_PARTS] = {}, *b[K82_ADAPTER_PARTS] = {}, *scale = nullptr, *gain[2] = {}, *offset[2] = {};
+};
+constexpr int kMaxAdapters = 1024;
 
 enum { FAM_CONV22 = 0, FAM_CONV14, FAM_LSTM, FAM_STATS, FAM_ATTN, FAM_ISTFT, FAM_SRC, FAM_OTHER, FAM_GATHER, NFAM };
 const char* const kFamNames[NFAM] = {"conv_mfma_2x2", "conv_mfma_1x4", "lstm", "instnorm", "attention", "istft", "source", "other", "gather"};
@@ -196,6 +204,7 @@ struct K82Weights {
     float *lin_w, *lin_b; ConvW nconv0, nconv1, ups0, ups1, conv_post;
     ResBlock1W nres[2], rb[6];
     float *sfc_pros_w, *sfc_pros_b, *sfc_dec_w, *sfc_dec_b; int Gp = 0, Gd = 0;
+    Adapters ad;
 };
 }  // namespace
 
@@ -211,6 +220,9 @@ struct k82_handle : K82Weights {
     std::vector<void*> wallocs;        // device weight allocations
     k82_handle* parent = nullptr;      // k82_fork: the handle whose weights this one reads (it must outlive this one)
     std::atomic<int> forks{0};         // live handles forked from this one
+
+    // which of the adapters have a part (K82_ADAPTER_*) / a norm of their own: host side of K82Weights::ad
+    std::vector<uint8_t> ad_part[K82_ADAPTER_PARTS], ad_norm[2];
 
     unsigned char* scratch = nullptr;  // this device's copy of the static scratch array (k82_pcm16_static)
 
@@ -887,6 +899,124 @@ struct k82_handle : K82Weights {
         }
     }
 
+    // ------------------------------------------------------------------ adapters
+    static void adapter_dims(const k82_config& cfg, int part, int* cin, int* cout) {
+        *cin = part == K82_ADAPTER_FFN_OUTPUT ? cfg.bert_inter : cfg.bert_hidden;
+        *cout = part == K82_ADAPTER_FFN ? cfg.bert_inter : cfg.bert_hidden;
+    }
+    void set_adapters(const k82_adapter* v, int n) {
+        REQUIRE(finalized, K82_ESTATE, "k82_finalize has not been called");
+        REQUIRE(!parent && forks.load() == 0, K82_ESTATE, "k82_set_adapters: forks read the adapters; destroy them first (and set adapters on the handle that owns the weights)");
+        REQUIRE(n >= 0 && n <= kMaxAdapters && (n == 0 || v), K82_EINVAL, "k82_set_adapters holds 0 to 1024 adapters");
+        Adapters t;
+        std::vector<uint8_t> part[K82_ADAPTER_PARTS], norm[2];
+        t.n = n;
+        for (int i = 0; i < n; ++i) {
+            bool any = false;
+            for (int p = 0; p < K82_ADAPTER_PARTS; ++p) {
+                REQUIRE(!v[i].a[p] == !v[i].b[p], K82_EINVAL, "adapter " + std::to_string(i) + ": a and b of a part come together");
+                any |= v[i].a[p] != nullptr;
+                part[p].push_back(v[i].a[p] != nullptr);
+            }
+            for (int m = 0; m < 2; ++m) {
+                REQUIRE(!v[i].gain[m] == !v[i].offset[m], K82_EINVAL, "adapter " + std::to_string(i) + ": gain and offset come together");
+                norm[m].push_back(v[i].gain[m] != nullptr);
+            }
+            REQUIRE(!any || (v[i].rank >= 1 && v[i].rank <= K82_LORA_MAX_RANK), K82_EINVAL, "adapter " + std::to_string(i) + ": rank must be in [1, 128]");
+            REQUIRE(!any || std::isfinite(v[i].scale), K82_EINVAL, "adapter " + std::to_string(i) + ": scale must be finite");
+            if (any) t.rank = std::max(t.rank, v[i].rank);
+        }
+        t.rank = ru(t.rank, 4);                // whole 16-byte loads
+        std::vector<float> all;                // the image of one allocation
+        size_t at_a[K82_ADAPTER_PARTS], at_b[K82_ADAPTER_PARTS], at_g[2], at_o[2];
+        const size_t D = cfg.bert_hidden;
+        auto grow = [&](size_t k) { const size_t at = all.size(); all.resize(at + (k + 63) / 64 * 64, 0.f); return at; };
+        for (int p = 0; p < K82_ADAPTER_PARTS; ++p) {
+            int cin, cout;
+            adapter_dims(cfg, p, &cin, &cout);
+            at_a[p] = grow((size_t)n * t.rank * cin);
+            at_b[p] = grow((size_t)n * t.rank * cout);
+            for (int i = 0; i < n; ++i) {
+                if (!part[p][i]) continue;
+                const int r = v[i].rank;
+                std::copy(v[i].a[p], v[i].a[p] + (size_t)r * cin, all.begin() + at_a[p] + (size_t)i * t.rank * cin);
+                for (int o = 0; o < cout; ++o) std::copy(v[i].b[p] + (size_t)o * r, v[i].b[p] + (size_t)(o + 1) * r, all.begin() + at_b[p] + ((size_t)i * cout + o) * t.rank);
+            }
+        }
+        const size_t at_s = grow(n);
+        for (int i = 0; i < n; ++i) all[at_s + i] = v[i].scale;
+        for (int m = 0; m < 2; ++m) {
+            at_g[m] = grow((size_t)n * D);
+            at_o[m] = grow((size_t)n * D);
+            for (int i = 0; i < n; ++i)
+                if (norm[m][i]) {
+                    std::copy(v[i].gain[m], v[i].gain[m] + D, all.begin() + at_g[m] + (size_t)i * D);
+                    std::copy(v[i].offset[m], v[i].offset[m] + D, all.begin() + at_o[m] + (size_t)i * D);
+                }
+        }
+        if (n) {
+            float* mem = nullptr;
+            if (hipMalloc((void**)&mem, all.size() * sizeof(float)) != hipSuccess) {
+                (void)hipGetLastError();
+                throw K82Error(K82_ENOMEM, "hipMalloc of " + std::to_string(all.size() * sizeof(float)) + " bytes failed (adapters)");
+            }
+            t.mem = (char*)mem;
+            if (hipMemcpy(mem, all.data(), all.size() * sizeof(float), hipMemcpyHostToDevice) != hipSuccess) {
+                (void)hipFree(mem);
+                throw K82Error(K82_EHIP, "copy of the adapters failed");
+            }
+            for (int p = 0; p < K82_ADAPTER_PARTS; ++p) { t.a[p] = mem + at_a[p]; t.b[p] = mem + at_b[p]; }
+            t.scale = mem + at_s;
+            for (int m = 0; m < 2; ++m) { t.gain[m] = mem + at_g[m]; t.offset[m] = mem + at_o[m]; }
+        }
+        (void)hipDeviceSynchronize();          // nothing reads the old ones any more
+        if (ad.mem) (void)hipFree(ad.mem);
+        ad = t;
+        for (int p = 0; p < K82_ADAPTER_PARTS; ++p) ad_part[p].swap(part[p]);
+        for (int m = 0; m < 2; ++m) ad_norm[m].swap(norm[m]);
+        have_phase1 = false;
+    }
+    // The sentences of the batch as segments of the packed token axis: for a Linear every one, -1 without a part of its own; for
+    // a norm those with one of their own alone.  Empty: nobody has.
+    struct Cut { std::vector<int64_t> off; std::vector<int32_t> index; k82_segments seg() const { return {off.data(), index.data(), (int32_t)index.size()}; } };
+    Cut adapter_cut(const int32_t* adapter, int part) const {
+        Cut c;
+        bool any = false;
+        for (int b = 0; b < B; ++b) {
+            const int k = adapter && adapter[b] >= 0 && ad_part[part][adapter[b]] ? adapter[b] : -1;
+            c.off.push_back(toff_h[b]);
+            c.index.push_back(k);
+            any |= k >= 0;
+        }
+        c.off.push_back(Ptot);
+        return any ? c : Cut();
+    }
+    std::vector<Cut> norm_cuts(const int32_t* adapter, int m) const {    // one cut for each run of neighbours with norms of their own
+        std::vector<Cut> v;
+        for (int b = 0; b < B; ++b) {
+            if (!adapter || adapter[b] < 0 || !ad_norm[m][adapter[b]]) continue;
+            if (v.empty() || v.back().off.back() != toff_h[b]) { v.emplace_back(); v.back().off.push_back(toff_h[b]); }
+            v.back().off.push_back(toff_h[b] + lens_h[b]);
+            v.back().index.push_back(adapter[b]);
+        }
+        return v;
+    }
+    // y[cout][P] = act(y + scale_k B_k A_k x) for the sentences' own adapters (y already holds the shared Linear)
+    void adapt(const Cut& c, int part, const float* x, float* y, int act) {
+        if (c.index.empty()) return;
+        int cin, cout;
+        adapter_dims(cfg, part, &cin, &cout);
+        const k82_lora p{K82_F32, K82_COLS, act, cin, cout, ad.rank, ad.n, Ptot, x, Pp, y, Pp, y, Pp, ad.a[part], ad.b[part], ad.scale, nullptr};
+        timed(FAM_OTHER, 0, [&] { HIPCHK(op::launch(p, c.seg(), st)); });
+    }
+    void adapt_norm(const std::vector<Cut>& cuts, int m, const float* x, float* y) {
+        for (const Cut& c : cuts) {
+            const k82_layernorm p{K82_F32, K82_COLS, cfg.bert_hidden, ad.n, 1e-12f, Ptot, x, Pp, nullptr, 0, y, Pp,
+                                  ad.gain[m], ad.offset[m], nullptr, nullptr};
+            timed(FAM_OTHER, 0, [&] { HIPCHK(op::launch(p, c.seg(), st)); });
+        }
+    }
+
     // ------------------------------------------------------------------ phase 1
     template <class T> T* to_device(const T* src, size_t n, Arena& ar) {
         T* d = (T*)ar.alloc(n * sizeof(T));
@@ -905,15 +1035,15 @@ struct k82_handle : K82Weights {
         return at.type == hipMemoryTypeDevice;
     }
     void durations(const int64_t* ids, const int32_t* lens, int nb, int tmax, const float* ref_s, const float* speed,
-                   const int32_t* forced, int32_t* pred_dur, int64_t* n_frames) {
-        durations_once(ids, lens, nb, tmax, ref_s, speed, forced, pred_dur, n_frames);
+                   const int32_t* forced, const int32_t* adapter, int32_t* pred_dur, int64_t* n_frames) {
+        durations_once(ids, lens, nb, tmax, ref_s, speed, forced, adapter, pred_dur, n_frames);
         if (lstm_timed_out()) {           // same inputs, streaming BiLSTM kernel: same bits as an undisturbed split run
-            durations_once(ids, lens, nb, tmax, ref_s, speed, forced, pred_dur, n_frames);
+            durations_once(ids, lens, nb, tmax, ref_s, speed, forced, adapter, pred_dur, n_frames);
             REQUIRE(!lstm_timed_out(), K82_EHIP, "LSTM recurrence failed on the streaming kernel as well");
         }
     }
     void durations_once(const int64_t* ids, const int32_t* lens, int nb, int tmax, const float* ref_s, const float* speed,
-                        const int32_t* forced, int32_t* pred_dur, int64_t* n_frames) {
+                        const int32_t* forced, const int32_t* adapter, int32_t* pred_dur, int64_t* n_frames) {
         REQUIRE(finalized, K82_ESTATE, "k82_finalize has not been called");
         REQUIRE(nb >= 1 && tmax >= 2 && tmax <= K82_MAX_TOKENS, K82_EINVAL, "B must be >= 1 and 2 <= Tmax <= 512");
         REQUIRE(ids && lens && ref_s, K82_EINVAL, "ids, lens and ref_s must not be NULL");
@@ -924,6 +1054,9 @@ struct k82_handle : K82Weights {
                     const int64_t v = ids[(size_t)b * tmax + t];
                     REQUIRE(v >= 0 && v < cfg.n_token, K82_EINVAL, "token id " + std::to_string(v) + " outside [0, n_token) at sentence " + std::to_string(b) + ", position " + std::to_string(t));
                 }
+        if (adapter)
+            for (int b = 0; b < nb; ++b)
+                REQUIRE(adapter[b] >= -1 && adapter[b] < ad.n, K82_EINVAL, "adapter " + std::to_string(adapter[b]) + " of sentence " + std::to_string(b) + " is outside [-1, " + std::to_string(ad.n) + ")");
         begin_pass();
         std::vector<float> sp(nb, 1.0f);
         if (speed) for (int b = 0; b < nb; ++b) { REQUIRE(speed[b] > 0.f && std::isfinite(speed[b]), K82_EINVAL, "speed must be positive"); sp[b] = speed[b]; }
@@ -965,22 +1098,35 @@ struct k82_handle : K82Weights {
         float* ff = aT.f((size_t)I * P);
         auto lin = [&](const ConvW& w, const float* x, float* y) { return cp(w, x, 0, P, y, 0, P, lp, lp, 1, Ptot); };
         run_conv(lin(map_in, emb, h), nullptr);
+        Cut cut[K82_ADAPTER_PARTS];
+        std::vector<Cut> ncut[2];
+        if (adapter && ad.n) {
+            for (int i = 0; i < K82_ADAPTER_PARTS; ++i) cut[i] = adapter_cut(adapter, i);
+            for (int m = 0; m < 2; ++m) ncut[m] = norm_cuts(adapter, m);
+        }
         for (int layer = 0; layer < cfg.bert_layers; ++layer) {
             run_conv(lin(qkv, h, qkvb), nullptr);
+            for (int i = 0; i < 3; ++i) adapt(cut[i], i, h, qkvb + (size_t)i * D * P, K82_ACT_NONE);
             double aw = 0;
             for (int b = 0; b < nb; ++b) aw += 4.0 * D * (double)lens[b] * lens[b];
             timed(FAM_ATTN, aw, [&] { launch_attention(qkvb, 0, P, ctx, 0, P, lt, cfg.bert_heads, nb, tmax, st); });
             ConvP pd = lin(attn_dense, ctx, tmp);
             pd.res = h; pd.rbs = 0; pd.rpitch = P;
             run_conv(pd, nullptr);
+            adapt(cut[K82_ADAPTER_DENSE], K82_ADAPTER_DENSE, ctx, tmp, K82_ACT_NONE);
             timed(FAM_OTHER, 0, [&] { launch_layernorm_cols(tmp, nullptr, h1, 0, 0, P, lt, D, nb, tmax, 1e-12f, ln_attn.w, ln_attn.b, nullptr, 0, 0, 1.0f, st); });
+            adapt_norm(ncut[0], 0, tmp, h1);
             ConvP pf = lin(ffn, h1, ff);
-            pf.out_act = OACT_GELU_NEW;
+            // (an adapter adds in front of the activation, which then moves behind it, for every sentence: same formula)
+            if (cut[K82_ADAPTER_FFN].index.empty()) pf.out_act = OACT_GELU_NEW;
             run_conv(pf, nullptr);
+            adapt(cut[K82_ADAPTER_FFN], K82_ADAPTER_FFN, h1, ff, K82_ACT_GELU_NEW);
             ConvP po = lin(ffn_out, ff, tmp);
             po.res = h1; po.rbs = 0; po.rpitch = P;
             run_conv(po, nullptr);
+            adapt(cut[K82_ADAPTER_FFN_OUTPUT], K82_ADAPTER_FFN_OUTPUT, ff, tmp, K82_ACT_NONE);
             timed(FAM_OTHER, 0, [&] { launch_layernorm_cols(tmp, nullptr, h, 0, 0, P, lt, D, nb, tmax, 1e-12f, ln_full.w, ln_full.b, nullptr, 0, 0, 1.0f, st); });
+            adapt_norm(ncut[1], 1, tmp, h);
         }
         tap_packed("bert_out", h, D);
 
@@ -1362,6 +1508,8 @@ int k82_fork(k82_handle* parent, k82_handle** out) {
         HIPCHK(hipSetDevice(h->device));
         HIPCHK(hipStreamCreateWithFlags(&h->own_stream, hipStreamNonBlocking));
         static_cast<K82Weights&>(*h) = static_cast<const K82Weights&>(*parent);
+        for (int i = 0; i < K82_ADAPTER_PARTS; ++i) h->ad_part[i] = parent->ad_part[i];
+        for (int i = 0; i < 2; ++i) h->ad_norm[i] = parent->ad_norm[i];
         h->scratch = parent->scratch;
         h->cus = parent->cus;
         h->kflush_div = parent->kflush_div; h->dec_ksplit = parent->dec_ksplit; h->splitk_on = parent->splitk_on; h->skcap = parent->skcap;
@@ -1403,6 +1551,7 @@ int k82_destroy(k82_handle* h) {
         (void)hipSetDevice(h->device);
         (void)hipDeviceSynchronize();
         for (void* p : h->wallocs) (void)hipFree(p);
+        if (!h->parent && h->ad.mem) (void)hipFree(h->ad.mem);
         h->aT.release();
         h->aF.release();
         for (auto e : h->evpool) (void)hipEventDestroy(e);
@@ -1432,7 +1581,17 @@ int k82_finalize(k82_handle* h) {
 
 int k82_durations(k82_handle* h, const int64_t* ids, const int32_t* lens, int B, int Tmax, const float* ref_s,
                   const float* speed, const int32_t* forced_dur, int32_t* pred_dur, int64_t* n_frames, void* stream) {
-    return guarded(h, stream, [&] { h->durations(ids, lens, B, Tmax, ref_s, speed, forced_dur, pred_dur, n_frames); });
+    return guarded(h, stream, [&] { h->durations(ids, lens, B, Tmax, ref_s, speed, forced_dur, nullptr, pred_dur, n_frames); });
+}
+
+int k82_durations_adapted(k82_handle* h, const int64_t* ids, const int32_t* lens, int B, int Tmax, const float* ref_s,
+                          const float* speed, const int32_t* forced_dur, const int32_t* adapter, int32_t* pred_dur,
+                          int64_t* n_frames, void* stream) {
+    return guarded(h, stream, [&] { h->durations(ids, lens, B, Tmax, ref_s, speed, forced_dur, adapter, pred_dur, n_frames); });
+}
+
+int k82_set_adapters(k82_handle* h, const k82_adapter* adapters, int32_t n) {
+    return guarded(h, nullptr, [&] { h->set_adapters(adapters, n); });
 }
 
 int k82_decode(k82_handle* h, const k82_noise* noise, float* audio, int64_t capacity, int64_t* audio_off, void* stream) {
@@ -1443,7 +1602,7 @@ int k82_synthesize(k82_handle* h, const int64_t* ids, const int32_t* lens, int B
                    const float* speed, const k82_noise* noise, int32_t* pred_dur, float* audio, int64_t capacity,
                    int64_t* audio_off, void* stream) {
     return guarded(h, stream, [&] {
-        h->durations(ids, lens, B, Tmax, ref_s, speed, nullptr, pred_dur, nullptr);
+        h->durations(ids, lens, B, Tmax, ref_s, speed, nullptr, nullptr, pred_dur, nullptr);
         h->decode(noise, audio, capacity, audio_off);
     });
 }

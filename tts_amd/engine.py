@@ -78,6 +78,7 @@ class Engine(Operators):
         child._pending = None
         child.config, child.device = self.config, self.device
         child._parent = self
+        child._adapters = dict(getattr(self, "_adapters", {}))
         child._forks = []
         child.h = C.c_void_p()
         with self._lock:
@@ -111,6 +112,33 @@ class Engine(Operators):
             self._pending = None
             self._check(self.lib.k82_reserve(self.h, int(batch), int(tokens), int(frames)))
             self._reserved = (max(want[0], have[0]), max(want[1], have[1]))
+
+    def set_adapters(self, adapters):
+        """k82_set_adapters: ``{name: tts_amd.Adapter}`` replaces the adapters of this engine (and of every front door that
+        shares it); ``durations(adapters=[name or None, ...])`` picks one for each sentence.  Call it before ``fork()``:
+        forks inherit what their parent holds, and while they live it is refused."""
+        from .adapters import Adapter
+        names = list(adapters)
+        for n in names:
+            if not isinstance(adapters[n], Adapter):
+                raise TypeError(f"adapter {n!r} is not a tts_amd.Adapter")
+        table = (_lib.K82Adapter * max(1, len(names)))(*[adapters[n].c_struct() for n in names])
+        with self._lock:
+            self._pending = None
+            self._check(self.lib.k82_set_adapters(self.h, table, len(names)))
+            self._adapters = {n: i for i, n in enumerate(names)}
+
+    def _adapter_indices(self, adapters, B):
+        """names / None of a batch -> host i32[B] (the caller holds the lock), or None."""
+        if adapters is None:
+            return None
+        if len(adapters) != B:
+            raise ValueError(f"adapters names {len(adapters)} sentences, the batch has {B}")
+        have = getattr(self, "_adapters", {})
+        unknown = [a for a in adapters if a is not None and a not in have]
+        if unknown:
+            raise KeyError(f"adapter {unknown[0]!r} not found; set_adapters() holds {sorted(have)[:8]}")
+        return np.array([-1 if a is None else have[a] for a in adapters], dtype=np.int32)
 
     # ------------------------------------------------------------------ plumbing
     def close(self):
@@ -147,8 +175,9 @@ class Engine(Operators):
             ids[b, 1:1 + len(x)] = np.asarray(x, dtype=np.int64)
         return ids, lens
 
-    def durations(self, ids, lens, ref_s, speed=None, forced_dur=None, stream=None):
-        """Phase 1.  Returns (pred_dur i32[B,Tmax], n_frames i64[B])."""
+    def durations(self, ids, lens, ref_s, speed=None, forced_dur=None, stream=None, adapters=None):
+        """Phase 1.  Returns (pred_dur i32[B,Tmax], n_frames i64[B]).  ``adapters``: a name known to ``set_adapters`` or
+        None for each sentence."""
         lens = np.ascontiguousarray(lens, dtype=np.int32)
         B = lens.shape[0]
         if isinstance(ids, np.ndarray):
@@ -164,8 +193,9 @@ class Engine(Operators):
         nfr = np.zeros((B,), dtype=np.int64)
         with self._lock:
             self._pending = None
-            self._check(self.lib.k82_durations(self.h, _ptr(ids), _ptr(lens), B, tmax, _ptr(ref_s), _ptr(sp), _ptr(fd),
-                                               _ptr(pred), _ptr(nfr), _ptr(stream)))
+            ad = self._adapter_indices(adapters, B)
+            self._check(self.lib.k82_durations_adapted(self.h, _ptr(ids), _ptr(lens), B, tmax, _ptr(ref_s), _ptr(sp),
+                                                       _ptr(fd), _ptr(ad), _ptr(pred), _ptr(nfr), _ptr(stream)))
             self._pending = (threading.get_ident(), nfr)
         return pred, nfr
 
@@ -206,11 +236,11 @@ class Engine(Operators):
             self._check(self.lib.k82_decode(self.h, C.byref(ns), _ptr(ptr), int(cap), _ptr(off), _ptr(stream)))
             return None, off
 
-    def synthesize(self, id_lists, ref_s, speed=None, noise=None, seeds=None):
+    def synthesize(self, id_lists, ref_s, speed=None, noise=None, seeds=None, adapters=None):
         """list of id lists -> list of f32 audio arrays (+ pred_dur).  Atomic with respect to other threads."""
         ids, lens = self.pack(id_lists)
         with self.session():
-            pred, _ = self.durations(ids, lens, ref_s, speed)
+            pred, _ = self.durations(ids, lens, ref_s, speed, adapters=adapters)
             audio, off = self.decode(noise=noise, seeds=seeds)
         return [audio[off[b]:off[b + 1]] for b in range(len(id_lists))], pred
 

@@ -124,11 +124,12 @@ class Kokoro:
         return id_lists, rows
 
     def create_batch(self, texts, voice, speed: float = 1.0, lang: str = "en-us", is_phonemes: bool = False,
-                     trim: bool = True):
+                     trim: bool = True, adapter=None):
         """``[create(t, ...) for t in texts]`` as ONE scheduled engine pass (all chunks of all texts are
         bucketed and batched together).  Not in kokoro_onnx: it is what the read-aloud look-ahead window
         (tts_amd/readaloud.py) and whole-chapter export use, because on the GPU a batch costs about what one
-        sentence does.  Same validation, chunking, style-row and trim rules as ``create``."""
+        sentence does.  Same validation, chunking, style-row and trim rules as ``create``.  ``adapter``: the name of an
+        adapter of ``engine.set_adapters`` (tts_amd/adapters.py), or a list with a name or None for each text."""
         assert 0.5 <= speed <= 2.0, "Speed should be between 0.5 and 2.0"
         if isinstance(voice, str):
             voice = self.get_voice_style(voice)
@@ -140,7 +141,13 @@ class Kokoro:
             rows += rs
             owner += [ti] * len(ids)
         seeds = [_content_seed(ids) for ids in id_lists]
-        res = self.synth.synthesize(id_lists, rows, speeds=[float(speed)] * len(id_lists), seeds=seeds)
+        more = {}
+        if adapter is not None:
+            names = [adapter] * len(texts) if isinstance(adapter, str) else list(adapter)
+            if len(names) != len(texts):
+                raise ValueError(f"adapter names {len(names)} texts, there are {len(texts)}")
+            more["adapters"] = [names[ti] for ti in owner]
+        res = self.synth.synthesize(id_lists, rows, speeds=[float(speed)] * len(id_lists), seeds=seeds, **more)
         parts = [[] for _ in texts]
         for i, ti in enumerate(owner):
             a = res[i][0]
@@ -150,11 +157,12 @@ class Kokoro:
         return [(np.concatenate(p).astype(np.float32), SAMPLE_RATE) for p in parts]
 
     def create(self, text, voice, speed: float = 1.0, lang: str = "en-us", is_phonemes: bool = False,
-               trim: bool = True):
+               trim: bool = True, adapter=None):
         """-> (samples float32[N] in [-1, 1], 24000).  Same contract as the reference boundary
         (speech7.py:127): phonemize, chunk to <= 510 phonemes, synthesize each chunk with the
         style row ``voice[len(tokens)]``, optionally trim silence, concatenate."""
-        return self.create_batch([text], voice, speed, lang, is_phonemes, trim)[0]
+        more = {} if adapter is None else {"adapter": adapter}
+        return self.create_batch([text], voice, speed, lang, is_phonemes, trim, **more)[0]
 
 
 # ------------------------------------------------------------------------------ surface B

@@ -121,7 +121,7 @@ class BatchSynthesizer:
             e.close()
         self.engines = self.engines[:1]
 
-    def _run(self, id_lists, ref_rows, speeds, seeds, out, where, engine=None):
+    def _run(self, id_lists, ref_rows, speeds, seeds, out, where, engine=None, adapters=None):
         engine = engine or self.engine
         t0 = time.perf_counter()
         ids, lens = engine.pack(id_lists)
@@ -131,7 +131,8 @@ class BatchSynthesizer:
         # on one engine (epubviewer_06_latest_1_nov_2025_theme.py:407,692,715) interleave whole batches, never halves
         with engine.session():
             t0 = time.perf_counter()
-            pred, nfr = engine.durations(ids, lens, refs, speed=np.asarray(speeds, np.float32))
+            more = {} if adapters is None else {"adapters": adapters}
+            pred, nfr = engine.durations(ids, lens, refs, speed=np.asarray(speeds, np.float32), **more)
             self._add(s_durations=time.perf_counter() - t0)
             real, padded = int(nfr.sum()), int(nfr.max()) * len(id_lists)
             split = len(id_lists) > 1 and (real > self.frame_budget or padded > self.frame_pad_limit * real)
@@ -155,13 +156,15 @@ class BatchSynthesizer:
             h = len(order) // 2
             for part in (order[:h], order[h:]):
                 self._run([id_lists[k] for k in part], [ref_rows[k] for k in part], [speeds[k] for k in part],
-                          [seeds[k] for k in part], out, [where[k] for k in part], engine)
+                          [seeds[k] for k in part], out, [where[k] for k in part], engine,
+                          None if adapters is None else [adapters[k] for k in part])
             return
         for k, w in enumerate(where):
             out[w] = (audio[off[k]:off[k + 1]], pred[k, :lens[k]].copy())     # views of the batch buffer: no second copy
 
-    def synthesize(self, id_lists, ref_rows, speeds=None, seeds=None, indices=None):
-        """-> {index: (audio f32[600 F], pred_dur i32[T])} for ``indices`` (default: all)."""
+    def synthesize(self, id_lists, ref_rows, speeds=None, seeds=None, indices=None, adapters=None):
+        """-> {index: (audio f32[600 F], pred_dur i32[T])} for ``indices`` (default: all).  ``adapters``: a name known to
+        ``Engine.set_adapters`` or None for each sentence; sentences with and without share batches."""
         n = len(id_lists)
         indices = list(range(n)) if indices is None else list(indices)
         speeds = [1.0] * n if speeds is None else list(speeds)
@@ -172,7 +175,7 @@ class BatchSynthesizer:
 
         def run(batch, engine):
             self._run([id_lists[i] for i in batch], [ref_rows[i] for i in batch], [speeds[i] for i in batch],
-                      [seeds[i] for i in batch], out, batch, engine)
+                      [seeds[i] for i in batch], out, batch, engine, None if adapters is None else [adapters[i] for i in batch])
 
         if len(self.engines) == 1 or len(batches) < 2:
             for batch in batches:
