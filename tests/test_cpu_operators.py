@@ -143,7 +143,8 @@ def test_segments_class_refuses_what_is_not_a_cut():
 
 def test_python_face_refuses_before_the_library():
     ops = object.__new__(Operators)                              # no GPU here: a face without a handle
-    ops.device, ops.h = 0, C.c_void_p()
+    ops.device, ops.h, ops.lib = 0, C.c_void_p(), _lib.load()
+    ops._bind()
     x, a, b, s = torch.zeros(4, 8), torch.zeros(1, 2, 8), torch.zeros(1, 6, 2), torch.ones(1)
     with pytest.raises(ValueError, match="must be on cuda:0"):
         ops.op_lora(x, a, b, s)
@@ -152,39 +153,69 @@ def test_python_face_refuses_before_the_library():
     with pytest.raises(ValueError, match="must be on cuda:0"):
         ops.op_layernorm(x, torch.ones(1, 8), torch.ones(1, 8))
     with pytest.raises(TypeError, match="float32 or bfloat16"):
-        ops._dtype(x.half())
-    with pytest.raises(TypeError, match="b is"):
-        ops._dtype(x, b=b.bfloat16())
+        ops.op_lora(x.half(), a, b, s)
+    ops.device = -1                                              # (what get_device() says of this machine's tensors)
+    with pytest.raises(TypeError, match="b is torch.bfloat16"):
+        ops.op_lora(x, a, b.bfloat16(), s)
+    with pytest.raises(TypeError, match="scale is torch.float64"):
+        ops.op_lora(x, a, b, s.double())
+    with pytest.raises(TypeError, match="a must be a torch tensor"):
+        ops.op_lora(x, a.numpy(), b, s)
+    with pytest.raises(ValueError, match="act must be one of"):
+        ops.op_lora(x, a, b, s, act="relu")
     with pytest.raises(ValueError, match="two dimensions"):
-        ops._layout(x=x[None])
+        ops.op_lora(x[None], a, b, s)
     with pytest.raises(ValueError, match="share one layout"):
-        ops._layout(x=x, base=torch.zeros(6, 4).t())             # rows beside channel-first
+        ops.op_lora(x, a, b, s, base=torch.zeros(6, 4).t())      # rows beside channel-first
     with pytest.raises(ValueError, match="share one layout"):
-        ops._layout(x=torch.zeros(1, 8).expand(4, 8))            # rows that lie on each other
+        ops.op_lora(torch.zeros(1, 8).expand(4, 8), a, b, s)     # rows that lie on each other
     with pytest.raises(ValueError, match="share one layout"):
-        ops._layout(True, x=torch.zeros(8, 4).t())               # the backward pass takes rows
+        ops.op_lora_grad(torch.zeros(8, 4).t(), torch.zeros(4, 6), torch.zeros(4, 2), a, b, s)       # the backward pass takes rows
     with pytest.raises(ValueError, match="scale has shape"):
-        ops._factors(x, a, b, torch.ones(2))
+        ops.op_lora(x, a, b, torch.ones(2))
     with pytest.raises(ValueError, match="b has shape"):
-        ops._factors(x, a, torch.zeros(1, 6, 3), s)
+        ops.op_lora(x, a, torch.zeros(1, 6, 3), s)
     with pytest.raises(ValueError, match="x has shape"):
-        ops._factors(torch.zeros(4, 7), a, b, s)
+        ops.op_lora(torch.zeros(4, 7), a, b, s)
+    with pytest.raises(ValueError, match="base has shape"):
+        ops.op_lora(x, a, b, s, base=torch.zeros(4, 7))
     with pytest.raises(ValueError, match="contiguous"):
-        ops._factors(x, torch.zeros(1, 8, 2).transpose(1, 2), b, s)
+        ops.op_lora(x, torch.zeros(1, 8, 2).transpose(1, 2), b, s)
     with pytest.raises(ValueError, match="end at token 5"):
-        ops._segments(Segments([0, 5], [0]), 4)
+        ops.op_lora(x, a, b, s, Segments([0, 5], [0]))
     with pytest.raises(TypeError, match="Segments"):
-        ops._segments([0, 4], 4)
+        ops.op_lora(x, a, b, s, [0, 4])
+    with pytest.raises(ValueError, match="h has shape"):
+        ops.op_lora_grad(x, torch.zeros(4, 6), torch.zeros(4, 3), a, b, s)
+    with pytest.raises(ValueError, match="gain has shape"):
+        ops.op_layernorm(x, torch.ones(1, 7), torch.ones(1, 8))
+    with pytest.raises(ValueError, match="mean has shape"):
+        ops.op_layernorm_grad(x, x, torch.ones(1, 8), torch.ones(3), torch.ones(4))
+    # the library's own refusal comes through with its reason
+    with pytest.raises(ValueError, match="index 1 of segment 0"):
+        ops.op_lora_grad(x, torch.zeros(4, 6), torch.zeros(4, 2), a, b, s, Segments([0, 4], [1]))
+
+
+def test_packed_arguments_are_the_structs():
+    from tts_amd import operators as O
+    for packed, c in ((O._LORA, _lib.K82Lora), (O._LORA_GRAD, _lib.K82LoraGrad), (O._NORM, _lib.K82Layernorm), (O._NORM_GRAD, _lib.K82LayernormGrad)):
+        assert packed.size == C.sizeof(c)
+        fields = [n for n, _ in c._fields_]
+        values = list(range(1, len(fields) + 1))
+        s = c.from_buffer_copy(packed.pack(*values))
+        assert [int(getattr(s, n)) for n in fields] == values
 
 
 def test_layouts_of_single_tokens_and_channels_are_taken_either_way():
+    def layout(*t, rows_only=False):
+        return Operators._layout(rows_only, [("t", v, None) for v in t])
     one = torch.zeros(32, 32).t()[:1, :8]                        # one token, channel-first
-    assert Operators._layout(x=one) == (1, [32])
-    assert Operators._layout(x=one, base=torch.zeros(1, 6)) == (1, [32, 1])
-    assert Operators._layout(x=torch.zeros(1, 8)) == (0, [8])
-    assert Operators._layout(x=torch.zeros(5, 9)[:, 1:], base=None) == (0, [9, 0])
-    assert Operators._layout(x=torch.zeros(9, 32).t()[:5]) == (1, [32])
-    assert Operators._layout(x=torch.zeros(7, 3)[:, :1]) == (0, [3])
+    assert layout(one) == (1, [32])
+    assert layout(one, torch.zeros(1, 6)) == (1, [32, 1])
+    assert layout(torch.zeros(1, 8)) == (0, [8])
+    assert layout(torch.zeros(5, 9)[:, 1:], None) == (0, [9, 0])
+    assert layout(torch.zeros(9, 32).t()[:5]) == (1, [32])
+    assert layout(torch.zeros(7, 3)[:, :1]) == (0, [3])
 
 
 # ---------------------------------------------------------------------------------------------- adapters of voices

@@ -11,12 +11,20 @@ stride along the tokens: ``buffer[channels, pitch].t()``, the engine's own layou
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 
 from . import _lib, spec
 
 ACTS = {"none": 0, "gelu_new": 1}
+
+# The argument structs of include/k82.h as native byte strings (a small call is bound by the host: 0.6 us where filling a
+# ctypes.Structure takes 2); the ctypes forms in _lib.py have the same sizes.
+_LORA = struct.Struct("@7i4xqPqPqPqPPPP")
+_LORA_GRAD = struct.Struct("@5i4xqPqPqPPqPqPPPPP")
+_NORM = struct.Struct("@4if4xqPqPqPqPPPP")
+_NORM_GRAD = struct.Struct("@3i4xqPqPqPqPqPPPPP")
 
 
 def _cfg_struct(config):
@@ -33,18 +41,19 @@ class Segments:
     """The cut of a packed token axis: segment ``s`` holds the tokens ``offsets[s]:offsets[s + 1]`` and uses adapter (or
     gain) ``index[s]``; -1 is a sentence without an adapter.  Host data; keep it for as many calls as the batch makes."""
 
-    __slots__ = ("offsets", "index", "c", "lo", "hi")
+    __slots__ = ("offsets", "index", "c", "address", "lo", "hi")
 
     def __init__(self, offsets, index):
         self.offsets = np.array(offsets, dtype=np.int64)
         self.index = np.array(index, dtype=np.int32)
         if self.offsets.ndim != 1 or self.index.ndim != 1 or self.offsets.size != self.index.size + 1:
             raise ValueError("Segments: offsets holds one value more than index")
-        if (np.diff(self.offsets) < 0).any() or self.offsets[0] < 0:
+        if self.offsets[0] < 0 or (self.offsets[1:] < self.offsets[:-1]).any():
             raise ValueError("Segments: offsets must not be negative and must not decrease")
         self.offsets.flags.writeable = self.index.flags.writeable = False
         self.lo, self.hi = int(self.offsets[0]), int(self.offsets[-1])
         self.c = _lib.K82Segments(off=self.offsets.ctypes.data, index=self.index.ctypes.data, n=self.index.size)
+        self.address = C.addressof(self.c)
 
     @classmethod
     def of_lengths(cls, lengths, index):
@@ -53,6 +62,8 @@ class Segments:
 
 class Operators:
     """A handle of libk82.so for the operators alone (``k82_create`` without weights)."""
+
+    _torch = None
 
     def __init__(self, device=0):
         self.device = device
@@ -85,154 +96,162 @@ class Operators:
             pass
 
     # ------------------------------------------------------------------ arguments
-    def _stream(self):
+    def _bind(self):
+        """What every call needs: torch (never imported before a handle is) and the entry points for packed arguments."""
         import torch
-        # torch's default stream is handle 0, which the library takes for "the handle's own": name it hipStreamLegacy (1)
-        return torch.cuda.current_stream(self.device).cuda_stream or 1
+        self._torch = torch
+        # the handle alone where torch offers it: a Stream object costs a microsecond
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        self._codes = {torch.float32: 0, torch.bfloat16: 1}
+        vp, i64 = C.c_void_p, C.c_int64
+        forward, backward = C.CFUNCTYPE(C.c_int, vp, C.c_char_p, vp, vp), C.CFUNCTYPE(C.c_int, vp, C.c_char_p, vp, vp, i64, vp)
+        size = C.CFUNCTYPE(i64, C.c_char_p, vp)
+        self._fn = {}
+        for op in ("lora", "layernorm"):
+            self._fn[op] = forward((f"k82_op_{op}", self.lib))
+            self._fn[op + "_grad"] = (backward((f"k82_op_{op}_grad", self.lib)), size((f"k82_op_{op}_grad_workspace", self.lib)))
+        return torch
 
-    def _on_gpu(self, **tensors):
-        for name, t in tensors.items():
+    def _stream(self):
+        # torch's default stream is handle 0, which the library takes for "the handle's own": name it hipStreamLegacy (1)
+        return self._raw_stream(self.device) or 1
+
+    def _placed(self, dtype, named):
+        """Every tensor is one of this GPU and of ``dtype``."""
+        dev = self.device
+        for name, t in named:
             if t is None:
                 continue
-            if not hasattr(t, "data_ptr"):
-                raise TypeError(f"{name} must be a torch tensor on the GPU")
-            if not t.is_cuda or t.get_device() != self.device:
-                raise ValueError(f"{name} must be on cuda:{self.device}, it is on {t.device}")
+            try:
+                at, dt = t.get_device(), t.dtype
+            except AttributeError:
+                raise TypeError(f"{name} must be a torch tensor on the GPU") from None
+            if at != dev:
+                raise ValueError(f"{name} must be on cuda:{dev}, it is on {t.device}")
+            if dt is not dtype:
+                raise TypeError(f"{name} is {dt}, {dtype} is needed")
 
-    @staticmethod
-    def _dtype(x, **others):
-        import torch
-        code = {torch.float32: 0, torch.bfloat16: 1}.get(x.dtype)
+    def _code(self, x):
+        code = self._codes.get(getattr(x, "dtype", None))
         if code is None:
+            if not hasattr(x, "data_ptr"):
+                raise TypeError("x must be a torch tensor on the GPU")
             raise TypeError(f"float32 or bfloat16 tensors are needed, x is {x.dtype}")
-        for name, t in others.items():
-            if t is not None and t.dtype != x.dtype:
-                raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}")
         return code
 
     @staticmethod
-    def _layout(rows_only=False, **tensors):
-        """-> (layout, [ld of each tensor]) of [tokens, channels] tensors that share one layout."""
-        rows, cols, lds = True, not rows_only, []
-        for name, t in tensors.items():
+    def _layout(rows_only, shapes):
+        """-> (layout, [ld of each]) of [tokens, channels] tensors that share one layout; shapes: (name, tensor or None,
+        wanted shape or None)."""
+        rows, cols, found = True, not rows_only, []
+        for name, t, want in shapes:
             if t is None:
+                found.append(None)
                 continue
-            if t.dim() != 2:
-                raise ValueError(f"{name} must have two dimensions [tokens, channels], it has {t.dim()}")
-            (n, c), (sn, sc) = t.shape, t.stride()
-            rows &= (sc == 1 or c == 1) and (n <= 1 or sn >= c)
-            cols &= (sn == 1 or n == 1) and (c <= 1 or sc >= n)
-        if not rows and not cols:
-            raise ValueError("tensors must share one layout: unit stride along the channels" + (
-                "" if rows_only else " (or along the tokens: channel-first)") + " and rows that do not overlap")
-        for t in tensors.values():
-            if t is None:
-                lds.append(0)
-            elif rows:
-                lds.append(t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1]))
-            else:
-                lds.append(t.stride(1) if t.shape[1] > 1 else max(1, t.shape[0]))
-        return (0 if rows else 1), lds
-
-    @staticmethod
-    def _like(name, t, shape):
-        if t is not None and tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, {tuple(shape)} is needed")
-
-    @staticmethod
-    def _contiguous(**tensors):
-        for name, t in tensors.items():
-            if t is not None and not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
-
-    @staticmethod
-    def _out(x, channels, cols, seg):
-        """A new [tokens, channels] tensor in the layout of x; zero where no segment will write."""
-        import torch
-        n = x.shape[0]
-        new = torch.empty if seg.lo == 0 and seg.hi == n else torch.zeros
+            shape = t.shape
+            if len(shape) != 2:
+                raise ValueError(f"{name} must have two dimensions [tokens, channels], it has {len(shape)}")
+            if want is not None and shape != want:
+                raise ValueError(f"{name} has shape {tuple(shape)}, {tuple(want)} is needed")
+            n, c = shape
+            sn, sc = t.stride()
+            rows = rows and (sc == 1 or c == 1) and (n <= 1 or sn >= c)
+            cols = cols and (sn == 1 or n == 1) and (c <= 1 or sc >= n)
+            found.append((n, c, sn, sc))
+        if rows:
+            return 0, [0 if v is None else v[2] if v[0] > 1 else max(1, v[1]) for v in found]
         if cols:
-            return new((channels, max(1, (n + 31) // 32 * 32)), dtype=x.dtype, device=x.device).t()[:n]
-        return new((n, channels), dtype=x.dtype, device=x.device)
+            return 1, [0 if v is None else v[3] if v[1] > 1 else max(1, v[0]) for v in found]
+        raise ValueError("tensors must share one layout: unit stride along the channels" + (
+            "" if rows_only else " (or along the tokens: channel-first)") + " and rows that do not overlap")
+
+    @staticmethod
+    def _need(name, t, shape):
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, {shape} is needed")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+
+    def _out(self, x, n, channels, cols, full):
+        """A new [tokens, channels] tensor in the layout of x and its ld; zero where no segment will write."""
+        new = self._torch.empty if full else self._torch.zeros
+        if cols:
+            ld = max(32, (n + 31) // 32 * 32)
+            return new((channels, ld), dtype=x.dtype, device=x.device).t()[:n], ld
+        return new((n, channels), dtype=x.dtype, device=x.device), channels
 
     @staticmethod
     def _segments(seg, n):
         if seg is None:
-            seg = Segments([0, n], [0])
-        elif not isinstance(seg, Segments):
+            return Segments([0, n], [0])
+        if not isinstance(seg, Segments):
             raise TypeError("seg must be a Segments (or None: every token uses index 0)")
         if seg.hi > n:
             raise ValueError(f"the segments end at token {seg.hi}, the tensors hold {n}")
         return seg
 
-    def _factors(self, x, a, b, scale):
-        import torch
+    def _factors(self, a, b, scale):
         if a.dim() != 3 or b.dim() != 3:
             raise ValueError("a is [adapters, rank, cin] and b [adapters, cout, rank]")
         n, rank, cin = a.shape
         cout = b.shape[1]
-        self._like("b", b, (n, cout, rank))
-        self._like("scale", scale, (n,))
-        if scale.dtype != torch.float32:
-            raise TypeError(f"scale must be float32, it is {scale.dtype}")
-        self._contiguous(a=a, b=b, scale=scale)
-        self._like("x", x, (x.shape[0], cin))
+        self._need("b", b, (n, cout, rank))
+        self._need("scale", scale, (n,))
+        if not a.is_contiguous():
+            raise ValueError("a must be contiguous")
         return n, rank, cin, cout
 
     # ------------------------------------------------------------------ low-rank adapters
     def op_lora(self, x, a, b, scale, seg=None, base=None, act="none", out=None, keep=False):
         """k82_op_lora: ``act(base + scale[k] * (x @ a[k].T) @ b[k].T)`` with ``k`` the adapter of the token's segment
-        (-1: ``act(base)``).  ``base``: the shared projection's output, which ``out`` may be.  ``keep``: returns
-        ``(y, h)`` with ``h = x @ a[k].T`` in float32, which ``op_lora_grad`` takes."""
-        import torch
-        self._on_gpu(x=x, a=a, b=b, scale=scale, base=base, out=out)
+        (-1: ``act(base)``).  ``a`` [adapters, rank, cin], ``b`` [adapters, cout, rank], ``scale`` float32 [adapters].
+        ``base``: the shared projection's output, which ``out`` may be.  ``keep``: returns ``(y, h)`` with
+        ``h = x @ a[k].T`` in float32, which ``op_lora_grad`` takes."""
+        torch = self._torch or self._bind()
+        code, dt, f32 = self._code(x), x.dtype, torch.float32
+        self._placed(dt, (("x", x), ("a", a), ("b", b), ("base", base), ("out", out)))
+        self._placed(f32, (("scale", scale),))
         if act not in ACTS:
             raise ValueError(f"act must be one of {sorted(ACTS)}, not {act!r}")
-        dtype = self._dtype(x, a=a, b=b, base=base, out=out)
-        layout, (ldx, ldbase, ldy) = self._layout(x=x, base=base, out=out)
-        n, rank, cin, cout = self._factors(x, a, b, scale)
+        n, rank, cin, cout = self._factors(a, b, scale)
         tokens = x.shape[0]
-        self._like("base", base, (tokens, cout))
-        self._like("out", out, (tokens, cout))
+        of_y = (tokens, cout)
+        layout, (ldx, ldbase, ldy) = self._layout(False, (("x", x, (tokens, cin)), ("base", base, of_y), ("out", out, of_y)))
         seg = self._segments(seg, tokens)
-        if out is None:
-            out = self._out(x, cout, layout, seg)
-            ldy = out.stride(layout) if out.shape[layout] > 1 else max(1, out.shape[1 - layout])
         full = seg.lo == 0 and seg.hi == tokens
-        h = (torch.empty if full else torch.zeros)((tokens, rank), dtype=torch.float32, device=x.device) if keep else None
-        p = _lib.K82Lora(dtype, layout, ACTS[act], cin, cout, rank, n, tokens, x.data_ptr(), ldx,
-                         None if base is None else base.data_ptr(), ldbase, out.data_ptr(), ldy, a.data_ptr(), b.data_ptr(),
-                         scale.data_ptr(), None if h is None else h.data_ptr())
-        self._check(self.lib.k82_op_lora(self.h, p, seg.c, self._stream()))
+        if out is None:
+            out, ldy = self._out(x, tokens, cout, layout, full)
+        h = (torch.empty if full else torch.zeros)((tokens, rank), dtype=f32, device=x.device) if keep else None
+        p = _LORA.pack(code, layout, ACTS[act], cin, cout, rank, n, tokens, x.data_ptr(), ldx, 0 if base is None else base.data_ptr(),
+                       ldbase, out.data_ptr(), ldy, a.data_ptr(), b.data_ptr(), scale.data_ptr(), 0 if h is None else h.data_ptr())
+        rc = self._fn["lora"](self.h, p, seg.address, self._stream())
+        if rc:
+            self._check(rc)
         return (out, h) if keep else out
 
     def op_lora_grad(self, x, dy, h, a, b, scale, seg=None, dx_base=None, dx=None):
         """k82_op_lora_grad -> ``(dx, da, db)``; ``dy`` is the gradient in front of the activation, ``h`` what
         ``op_lora(keep=True)`` returned, ``dx_base`` the shared projection's gradient (which ``dx`` may be).  ``da`` and
         ``db`` are float32 sums over the tokens in a fixed order, zero for an adapter without tokens."""
-        import torch
-        self._on_gpu(x=x, dy=dy, h=h, a=a, b=b, scale=scale, dx_base=dx_base, dx=dx)
-        dtype = self._dtype(x, dy=dy, a=a, b=b, dx_base=dx_base, dx=dx)
-        _, (ldx, lddy, ldbase, lddx) = self._layout(True, x=x, dy=dy, dx_base=dx_base, dx=dx)
-        n, rank, cin, cout = self._factors(x, a, b, scale)
+        torch = self._torch or self._bind()
+        code, dt, f32 = self._code(x), x.dtype, torch.float32
+        self._placed(dt, (("x", x), ("dy", dy), ("a", a), ("b", b), ("dx_base", dx_base), ("dx", dx)))
+        self._placed(f32, (("h", h), ("scale", scale)))
+        n, rank, cin, cout = self._factors(a, b, scale)
         tokens = x.shape[0]
-        self._like("dy", dy, (tokens, cout))
-        self._like("h", h, (tokens, rank))
-        if h.dtype != torch.float32:
-            raise TypeError(f"h must be float32, it is {h.dtype}")
-        self._contiguous(h=h)
-        self._like("dx_base", dx_base, (tokens, cin))
-        self._like("dx", dx, (tokens, cin))
+        of_x = (tokens, cin)
+        _, (ldx, lddy, ldbase, lddx) = self._layout(True, (("x", x, of_x), ("dy", dy, (tokens, cout)), ("dx_base", dx_base, of_x),
+                                                           ("dx", dx, of_x)))
+        self._need("h", h, (tokens, rank))
         seg = self._segments(seg, tokens)
         if dx is None:
-            dx = self._out(x, cin, 0, seg)
-            lddx = cin
-        da = torch.empty((n, rank, cin), dtype=torch.float32, device=x.device)
-        db = torch.empty((n, cout, rank), dtype=torch.float32, device=x.device)
-        p = _lib.K82LoraGrad(dtype, cin, cout, rank, n, tokens, x.data_ptr(), ldx, dy.data_ptr(), lddy, h.data_ptr(),
-                             None if dx_base is None else dx_base.data_ptr(), ldbase, dx.data_ptr(), lddx, a.data_ptr(),
-                             b.data_ptr(), scale.data_ptr(), da.data_ptr(), db.data_ptr())
-        self._with_workspace(self.lib.k82_op_lora_grad, self.lib.k82_op_lora_grad_workspace, p, seg, x)
+            dx, lddx = self._out(x, tokens, cin, 0, seg.lo == 0 and seg.hi == tokens)
+        da = torch.empty((n, rank, cin), dtype=f32, device=x.device)
+        db = torch.empty((n, cout, rank), dtype=f32, device=x.device)
+        p = _LORA_GRAD.pack(code, cin, cout, rank, n, tokens, x.data_ptr(), ldx, dy.data_ptr(), lddy, h.data_ptr(),
+                            0 if dx_base is None else dx_base.data_ptr(), ldbase, dx.data_ptr(), lddx, a.data_ptr(),
+                            b.data_ptr(), scale.data_ptr(), da.data_ptr(), db.data_ptr())
+        self._with_workspace("lora_grad", p, seg, x)
         return dx, da, db
 
     # ------------------------------------------------------------------ layer norm
@@ -240,66 +259,62 @@ class Operators:
         """k82_op_layernorm: ``(z - mean) * rstd * gain[k] + offset[k]`` over the channels of ``z = x + res``, ``gain`` and
         ``offset`` ``[gains, channels]``, ``k`` the index of the token's segment.  ``out`` may be ``x`` or ``res``.
         ``stats``: returns ``(y, mean, rstd)`` (float32), which ``op_layernorm_grad`` takes."""
-        import torch
-        self._on_gpu(x=x, gain=gain, offset=offset, res=res, out=out)
-        dtype = self._dtype(x, gain=gain, offset=offset, res=res, out=out)
-        layout, (ldx, ldres, ldy) = self._layout(x=x, res=res, out=out)
-        tokens, c = x.shape
+        torch = self._torch or self._bind()
+        code = self._code(x)
+        self._placed(x.dtype, (("x", x), ("gain", gain), ("offset", offset), ("res", res), ("out", out)))
+        shape = x.shape
+        layout, (ldx, ldres, ldy) = self._layout(False, (("x", x, None), ("res", res, shape), ("out", out, shape)))
+        tokens, c = shape
         gains = gain.shape[0]
-        self._like("gain", gain, (gains, c))
-        self._like("offset", offset, (gains, c))
-        self._contiguous(gain=gain, offset=offset)
-        self._like("res", res, (tokens, c))
-        self._like("out", out, (tokens, c))
+        self._need("gain", gain, (gains, c))
+        self._need("offset", offset, (gains, c))
         seg = self._segments(seg, tokens)
+        full = seg.lo == 0 and seg.hi == tokens
         if out is None:
-            out = self._out(x, c, layout, seg)
-            ldy = out.stride(layout) if out.shape[layout] > 1 else max(1, out.shape[1 - layout])
+            out, ldy = self._out(x, tokens, c, layout, full)
         mean = rstd = None
         if stats:
-            new = torch.empty if seg.lo == 0 and seg.hi == tokens else torch.zeros
+            new = torch.empty if full else torch.zeros
             mean, rstd = (new((tokens,), dtype=torch.float32, device=x.device) for _ in range(2))
-        p = _lib.K82Layernorm(dtype, layout, c, gains, eps, tokens, x.data_ptr(), ldx,
-                              None if res is None else res.data_ptr(), ldres, out.data_ptr(), ldy, gain.data_ptr(),
-                              offset.data_ptr(), None if mean is None else mean.data_ptr(),
-                              None if rstd is None else rstd.data_ptr())
-        self._check(self.lib.k82_op_layernorm(self.h, p, seg.c, self._stream()))
+        p = _NORM.pack(code, layout, c, gains, eps, tokens, x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldres,
+                       out.data_ptr(), ldy, gain.data_ptr(), offset.data_ptr(), 0 if mean is None else mean.data_ptr(),
+                       0 if rstd is None else rstd.data_ptr())
+        rc = self._fn["layernorm"](self.h, p, seg.address, self._stream())
+        if rc:
+            self._check(rc)
         return (out, mean, rstd) if stats else out
 
     def op_layernorm_grad(self, x, dy, gain, mean, rstd, seg=None, res=None, dx=None):
         """k82_op_layernorm_grad -> ``(dx, dgain, doffset)``: ``dx`` is the gradient of ``x`` and of ``res`` alike and may be
         ``dy``, ``x`` or ``res`` itself; ``dgain`` and ``doffset`` are float32 sums over the tokens in a fixed order."""
-        import torch
-        self._on_gpu(x=x, dy=dy, gain=gain, mean=mean, rstd=rstd, res=res, dx=dx)
-        dtype = self._dtype(x, dy=dy, gain=gain, res=res, dx=dx)
-        _, (ldx, ldres, lddy, lddx) = self._layout(True, x=x, res=res, dy=dy, dx=dx)
-        tokens, c = x.shape
+        torch = self._torch or self._bind()
+        code, f32 = self._code(x), torch.float32
+        self._placed(x.dtype, (("x", x), ("dy", dy), ("gain", gain), ("res", res), ("dx", dx)))
+        self._placed(f32, (("mean", mean), ("rstd", rstd)))
+        shape = x.shape
+        _, (ldx, ldres, lddy, lddx) = self._layout(True, (("x", x, None), ("res", res, shape), ("dy", dy, shape), ("dx", dx, shape)))
+        tokens, c = shape
         gains = gain.shape[0]
-        self._like("gain", gain, (gains, c))
-        self._like("dy", dy, (tokens, c))
-        self._like("res", res, (tokens, c))
-        self._like("dx", dx, (tokens, c))
-        for name, t in (("mean", mean), ("rstd", rstd)):
-            self._like(name, t, (tokens,))
-            if t.dtype != torch.float32:
-                raise TypeError(f"{name} must be float32, it is {t.dtype}")
-        self._contiguous(gain=gain, mean=mean, rstd=rstd)
+        self._need("gain", gain, (gains, c))
+        self._need("mean", mean, (tokens,))
+        self._need("rstd", rstd, (tokens,))
         seg = self._segments(seg, tokens)
         if dx is None:
-            dx = self._out(x, c, 0, seg)
-            lddx = c
-        dgain = torch.empty((gains, c), dtype=torch.float32, device=x.device)
-        doffset = torch.empty((gains, c), dtype=torch.float32, device=x.device)
-        p = _lib.K82LayernormGrad(dtype, c, gains, tokens, x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldres,
-                                  dy.data_ptr(), lddy, dx.data_ptr(), lddx, gain.data_ptr(), mean.data_ptr(),
-                                  rstd.data_ptr(), dgain.data_ptr(), doffset.data_ptr())
-        self._with_workspace(self.lib.k82_op_layernorm_grad, self.lib.k82_op_layernorm_grad_workspace, p, seg, x)
+            dx, lddx = self._out(x, tokens, c, 0, seg.lo == 0 and seg.hi == tokens)
+        dgain = torch.empty((gains, c), dtype=f32, device=x.device)
+        doffset = torch.empty((gains, c), dtype=f32, device=x.device)
+        p = _NORM_GRAD.pack(code, c, gains, tokens, x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldres,
+                            dy.data_ptr(), lddy, dx.data_ptr(), lddx, gain.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                            dgain.data_ptr(), doffset.data_ptr())
+        self._with_workspace("layernorm_grad", p, seg, x)
         return dx, dgain, doffset
 
-    def _with_workspace(self, call, size, p, seg, x):
-        import torch
-        need = size(p, seg.c)
+    def _with_workspace(self, op, p, seg, x):
+        call, size = self._fn[op]
+        need = size(p, seg.address)
         if need < 0:
             raise ValueError(f"k82 error {need}: {self.lib.k82_last_error(None).decode()}")
-        ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
-        self._check(call(self.h, p, seg.c, None if ws is None else ws.data_ptr(), need, self._stream()))
+        ws = self._torch.empty((need,), dtype=self._torch.uint8, device=x.device) if need else None
+        rc = call(self.h, p, seg.address, None if ws is None else ws.data_ptr(), need, self._stream())
+        if rc:
+            self._check(rc)
