@@ -164,8 +164,10 @@ constexpr int kPad = 4;                        // floats behind a row of the res
 // row a wave at a time.  The results cross LDS once more, so that base and y are read and written in whole lines.
 // blockIdx.y splits the output channels where there are few tokens; each part then computes h for itself, from cache.
 // EVEN: cin, cout and rank are multiples of a lane's 16 bytes, no place lies in part behind a row.
+// (waves_per_eu: without it the accumulators of four and eight rank tiles are copied through the second register file and one
+// wave less fits a SIMD; 65536 tokens 2048 -> 768 bf16 rank 64: 146 us, with it 137.)
 template <class T, int NW, int RT, int TT, bool EVEN>
-__global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lora p) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8 ? 2 : RT >= 4 ? 3 : 4))) void lora_rows_kernel(SegTable sg, k82_lora p) {
     constexpr int V = Vec<T>::N, K = 4 * V, S = sizeof(T), U = RT + TT > 4 ? 2 : 4;          // U: steps whose loads are in flight together
     constexpr int CH = 8 * V, MT = CH / 16, CK = Second<T, RT>::CHUNKS;          // channels, row tiles of B, chunks of a row of B
     constexpr int kTiles = most(RT + TT, MT * CK), kRow = CH + kPad;
@@ -273,17 +275,12 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
         for (int i = threadIdx.x; i < n; i += 64 * NW) p.h[t0 * p.rank + i] = 0.f;
     }
     for (; blk < blocks; blk += stride) {
-        raw4 now[2 * TT], tile[MT][CK];
+        raw4 now[2 * TT];
 #pragma unroll
         for (int i = 0; i < 2 * TT; ++i) now[i] = base[i];
         if (k >= 0) {
 #pragma unroll
             for (int i = 0; i < MT * CK; ++i) put_tile(own + i * 64, fac[i]);
-            wave_fence();
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int c = 0; c < CK; ++c) tile[m][c] = get_factor<T, RT>(own + (m * CK + c) * 64);
         }
         if (blk + stride < blocks) fetch(blk + stride);          // the next block is on its way while this one is multiplied
         const int n = p.cout - blk * CH - c8;
@@ -291,8 +288,14 @@ __global__ __launch_bounds__(64 * NW) void lora_rows_kernel(SegTable sg, k82_lor
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             if (k >= 0) {
+                wave_fence();
 #pragma unroll
-                for (int m = 0; m < MT; ++m) *(f4*)(result + col * kRow + 16 * m + 4 * g) = h[t].times(tile[m], f4{0.f, 0.f, 0.f, 0.f});
+                for (int m = 0; m < MT; ++m) {                   // (B's tiles are read for each t: registers for them would cost a wave)
+                    raw4 tile[CK];
+#pragma unroll
+                    for (int c = 0; c < CK; ++c) tile[c] = get_factor<T, RT>(own + (m * CK + c) * 64);
+                    *(f4*)(result + col * kRow + 16 * m + 4 * g) = h[t].times(tile, f4{0.f, 0.f, 0.f, 0.f});
+                }
                 wave_fence();
             }
 #pragma unroll
@@ -527,18 +530,20 @@ __device__ __forceinline__ void split3(const float (&v)[8], raw4& hi, raw4& mid,
 // Sums over tokens: part[chunk][r][cin + cout] = s_k sum_t v_t[r] z_t[c] with (v, z) = (g / s_k, x) for the first cin channels
 // and (h, dy) behind them.  A wave owns 128 channels of one of the two for all the tokens of a chunk.  The token axis is the
 // k of the product: f32 takes it as it lies (4 tokens an instruction), bf16 through the transpose in registers.
-template <class T, int RT>
+// More than 32 ranks are shares of blockIdx.z: their sums would leave one wave a SIMD, and the channels come from cache again.
+template <class T, int RT, bool EVEN>
 __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k82_lora_grad p, const float* gs, const float* scales, int used0, float* part) {
-    constexpr int V = Vec<T>::N, M = 8;                          // 16 x 16 tiles along the channels
+    constexpr int V = Vec<T>::N, M = 8, S = sizeof(T);           // M: 16 x 16 tiles along the channels
+    const int r0 = 32 * blockIdx.z;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int chunk = rt.chunk0[0] + (int)blockIdx.x, run = place(rt.chunk0, chunk);
+    const int chunk = rt.chunk0[0] + (int)blockIdx.y, run = place(rt.chunk0, chunk);
     const int u0 = rt.run_cum[run] + (chunk - rt.chunk0[run]) * rt.rows, u1 = min(u0 + rt.rows, rt.run_cum[run + 1]);
-    int slice = (int)blockIdx.y * kWaves + wave;
+    int slice = (int)blockIdx.x * kWaves + wave;
     const int nx = (p.cin + 127) / 128, ny = (p.cout + 127) / 128;
     if (slice >= nx + ny) return;
     const bool of_x = slice < nx;
     if (!of_x) slice -= nx;
-    const T* z = (const T*)(of_x ? p.x : p.dy);
+    const char* z = (const char*)(of_x ? p.x : p.dy);
     const int64_t ld = of_x ? p.ldx : p.lddy;
     const int width = of_x ? p.cin : p.cout, c0 = 128 * slice;
     const float* v = of_x ? gs : p.h;
@@ -547,60 +552,82 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
     for (int m = 0; m < M; ++m)
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[m][r] = f4{0.f, 0.f, 0.f, 0.f};
+    // 16 bytes of channel c on of a row; behind the row's end (EVEN: whole places) anything that is there, it is not stored
+    auto take = [&](const char* row, int c) -> raw4 {
+        if constexpr (EVEN) return load16(row, min(c, width - V) * S);
+        else return c < width ? load_part((const T*)row + c, width - c) : raw4{0u, 0u, 0u, 0u};
+    };
     int piece = place(rt.cum, u0);
     for (int u = u0; u < u1; ++piece) {                          // the pieces of a chunk, each a run of neighbouring tokens
         const int stop = min(u1, rt.cum[piece + 1]);
         const int64_t t0 = rt.start[piece] + (u - rt.cum[piece]);
         const int n = stop - u;
         u = stop;
+        const char* zp = z + t0 * ld * S;
+        const float* vp = v + t0 * p.rank;
         if constexpr (V == 8) {
-            const int c = c0 + 8 * col, left = width - c;
-            for (int i = 0; i < n; i += 32) {
+            auto step = [&](int i, auto whole) {                 // 32 tokens, 8 g + j in a lane; not whole: zeros behind the n-th
+                constexpr bool WHOLE = decltype(whole)::value;
                 raw4 raw[8], zt[8];
+                const raw4 zero = {0u, 0u, 0u, 0u};
+                float w[RT][8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int t = i + 8 * g + j;
-                    raw[j] = raw4{0u, 0u, 0u, 0u};
-                    if (t < n && left > 0) raw[j] = load_part(z + (t0 + t) * ld + c, left);
-                }
-                raw4 part3[RT][3];
+                    const int t = i + 8 * g + j, at = WHOLE ? t : min(t, n - 1);
+                    raw[j] = take(zp + at * ld * S, c0 + 8 * col);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    float w[8];
-                    const int at = min(16 * r + col, p.rank - 1);
+                    for (int r = 0; r < RT; ++r) w[r][j] = vp[at * p.rank + min(r0 + 16 * r + col, p.rank - 1)];
+                    if constexpr (!WHOLE) {
+                        raw[j] = t < n ? raw[j] : zero;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int t = i + 8 * g + j;
-                        w[j] = t < n ? v[(t0 + t) * p.rank + at] : 0.f;
+                        for (int r = 0; r < RT; ++r) w[r][j] = t < n ? w[r][j] : 0.f;
                     }
-                    split3(w, part3[r][0], part3[r][1], part3[r][2]);
                 }
                 transpose8(raw, zt);
 #pragma unroll
-                for (int m = 0; m < 8; ++m)
+                for (int r = 0; r < RT; ++r) {
+                    raw4 w3[3];
+                    split3(w[r], w3[0], w3[1], w3[2]);
+#pragma unroll
+                    for (int m = 0; m < 8; ++m)
+#pragma unroll
+                        for (int q = 2; q >= 0; --q) acc[m][r] = product<T>(zt[m], w3[q], acc[m][r]);
+                }
+            };
+            int i = 0;
+            for (; i + 32 <= n; i += 32) step(i, std::true_type());
+            if (i < n) step(i, std::false_type());
+        } else {
+            auto step = [&](int i, auto whole) {                 // 16 tokens, 4 j + g in instruction j
+                constexpr bool WHOLE = decltype(whole)::value;
+                raw4 raw[4][2];
+                const raw4 zero = {0u, 0u, 0u, 0u};
+                float w[RT][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int t = i + 4 * j + g, at = WHOLE ? t : min(t, n - 1);
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) raw[j][m] = take(zp + at * ld * S, c0 + 64 * m + 4 * col);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) w[r][j] = vp[at * p.rank + min(r0 + 16 * r + col, p.rank - 1)];
+                    if constexpr (!WHOLE) {
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) raw[j][m] = t < n ? raw[j][m] : zero;
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) w[r][j] = t < n ? w[r][j] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int r = 0; r < RT; ++r)
 #pragma unroll
-                        for (int q = 2; q >= 0; --q) acc[m][r] = product<T>(zt[m], part3[r][q], acc[m][r]);
-            }
-        } else {
-            for (int i = 0; i < n; i += 4) {
-                const int t = i + g;
-                raw4 raw[2];
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    const int c = c0 + 64 * m + 4 * col;
-                    raw[m] = raw4{0u, 0u, 0u, 0u};
-                    if (t < n && c < width) raw[m] = load_part(z + (t0 + t) * ld + c, width - c);
-                }
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const float w = t < n ? v[(t0 + t) * p.rank + min(16 * r + col, p.rank - 1)] : 0.f;
-#pragma unroll
-                    for (int m = 0; m < 8; ++m)
-                        acc[m][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw[m >> 2][m & 3]), w, acc[m][r], 0, 0, 0);
-                }
-            }
+                        for (int m = 0; m < 8; ++m)
+                            acc[m][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw[j][m >> 2][m & 3]), w[r][j], acc[m][r], 0, 0, 0);
+            };
+            int i = 0;
+            for (; i + 16 <= n; i += 16) step(i, std::true_type());
+            if (i < n) step(i, std::false_type());
         }
     }
     // row 4 g + i of tile m is the channel 8 (4 g + i) + m (bf16) or 64 (m / 4) + 4 (4 g + i) + m % 4 (f32)
@@ -608,8 +635,8 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
     float* out = part + (int64_t)chunk * p.rank * (p.cin + p.cout) + (of_x ? 0 : p.cin);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        if (16 * r + col >= p.rank) continue;
-        float* q = out + (int64_t)(16 * r + col) * (p.cin + p.cout);
+        if (r0 + 16 * r + col >= p.rank) continue;
+        float* q = out + (int64_t)(r0 + 16 * r + col) * (p.cin + p.cout);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -624,8 +651,15 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
 __global__ __launch_bounds__(256) void lora_reduce_kernel(ReduceTable rt, int cin, int cout, int rank, const float* part, float* da, float* db) {
     const int c = (int)blockIdx.x * 256 + (int)threadIdx.x, r = blockIdx.y, k = blockIdx.z;
     if (c >= cin + cout) return;
+    const int64_t step = (int64_t)rank * (cin + cout);
+    const float* q = part + (int64_t)rt.first[k] * step + (int64_t)r * (cin + cout) + c;
+    int n = rt.first[k + 1] - rt.first[k];
     float s = 0.f;
-    for (int i = rt.first[k]; i < rt.first[k + 1]; ++i) s += part[((int64_t)i * rank + r) * (cin + cout) + c];
+    for (; n >= 4; n -= 4, q += 4 * step) {                      // (four loads at once, added in order)
+        const float v0 = q[0], v1 = q[step], v2 = q[2 * step], v3 = q[3 * step];
+        s += v0; s += v1; s += v2; s += v3;
+    }
+    for (; n > 0; --n, q += step) s += *q;
     if (c < cin) da[((int64_t)(rt.base + k) * rank + r) * cin + c] = s;
     else db[((int64_t)(rt.base + k) * cout + (c - cin)) * rank + r] = s;
 }
@@ -673,7 +707,7 @@ template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::S
 int chunk_rows(const k82_lora_grad& p, int64_t tokens) {
     const int64_t slices = ((p.cin + 127) / 128 + (p.cout + 127) / 128 + kWaves - 1) / kWaves;
     const int64_t chunks = std::max<int64_t>(1, 512 / slices);
-    return (int)std::max<int64_t>(64, ((tokens + chunks - 1) / chunks + 31) / 32 * 32);
+    return (int)std::max<int64_t>(32, ((tokens + chunks - 1) / chunks + 31) / 32 * 32);
 }
 struct Layout { int64_t g, at, bt, scale, part, end; };         // bytes
 Layout layout(const k82_lora_grad& p, const k82_segments& s) {
@@ -718,12 +752,13 @@ template <class T> hipError_t backward(const k82_lora_grad& p, const k82_segment
                      p.dx_base, p.lddx_base, p.dx, p.lddx, bt, at, scale, g};
     OP_TRY(forward<T>(f, segs, st));
     const int slices = ((p.cin + 127) / 128 + (p.cout + 127) / 128 + kWaves - 1) / kWaves;
+    const bool even = p.cin % Vec<T>::N == 0 && p.cout % Vec<T>::N == 0;
     for (size_t i = 0; i < plan.tables.size(); ++i) {
         const RunTable& t = plan.tables[i];
-        OP_TRY(by_rank(p.rank, [&](auto rt) {
-            return op::run(lora_weight_kernel<T, decltype(rt)::value>, dim3(t.chunk0[t.runs] - t.chunk0[0], slices), dim3(64 * kWaves), 0, st, t, p,
-                           (const float*)g, (const float*)scale, first[i], part);
-        }));
+        const auto kernel = p.rank <= 16 ? (even ? lora_weight_kernel<T, 1, true> : lora_weight_kernel<T, 1, false>)
+                                         : (even ? lora_weight_kernel<T, 2, true> : lora_weight_kernel<T, 2, false>);
+        OP_TRY(op::run(kernel, dim3(slices, t.chunk0[t.runs] - t.chunk0[0], (p.rank + 31) / 32), dim3(64 * kWaves), 0, st, t, p, (const float*)g,
+                       (const float*)scale, first[i], part));
     }
     for (const ReduceTable& t : plan.reduce)
         OP_TRY(op::run(lora_reduce_kernel, dim3((p.cin + p.cout + 255) / 256, p.rank, t.n), dim3(256), 0, st, t, p.cin, p.cout, p.rank,
