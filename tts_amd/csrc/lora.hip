@@ -530,17 +530,20 @@ __device__ __forceinline__ void split3(const float (&v)[8], raw4& hi, raw4& mid,
 // Sums over tokens: part[chunk][r][cin + cout] = s_k sum_t v_t[r] z_t[c] with (v, z) = (g / s_k, x) for the first cin channels
 // and (h, dy) behind them.  A wave owns 128 channels of one of the two for all the tokens of a chunk.  The token axis is the
 // k of the product: f32 takes it as it lies (4 tokens an instruction), bf16 through the transpose in registers.
-// More than 32 ranks are shares of blockIdx.z: their sums would leave one wave a SIMD, and the channels come from cache again.
+// More than 32 ranks are shares of neighbouring workgroups (their sums would leave one wave a SIMD): the channels come from the
+// shared cache again, 65536 tokens 768 / 2048 rank 64 130 us, with the shares one after the other 173.
 template <class T, int RT, bool EVEN>
 __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k82_lora_grad p, const float* gs, const float* scales, int used0, float* part) {
     constexpr int V = Vec<T>::N, M = 8, S = sizeof(T);           // M: 16 x 16 tiles along the channels
-    const int r0 = 32 * blockIdx.z;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int chunk = rt.chunk0[0] + (int)blockIdx.y, run = place(rt.chunk0, chunk);
     const int u0 = rt.run_cum[run] + (chunk - rt.chunk0[run]) * rt.rows, u1 = min(u0 + rt.rows, rt.run_cum[run + 1]);
-    int slice = (int)blockIdx.x * kWaves + wave;
+    // waves of a workgroup: slices of 128 channels; from two rank shares on, two slices by two shares
+    const int shares = (p.rank + 31) / 32, pair = shares > 1 ? 2 : 1, groups = (shares + pair - 1) / pair, per = kWaves / pair;
+    const int share = (int)blockIdx.x % groups * pair + wave / per, r0 = 32 * share;
+    int slice = (int)blockIdx.x / groups * per + wave % per;
     const int nx = (p.cin + 127) / 128, ny = (p.cout + 127) / 128;
-    if (slice >= nx + ny) return;
+    if (slice >= nx + ny || share >= shares) return;
     const bool of_x = slice < nx;
     if (!of_x) slice -= nx;
     const char* z = (const char*)(of_x ? p.x : p.dy);
@@ -552,11 +555,15 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
     for (int m = 0; m < M; ++m)
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[m][r] = f4{0.f, 0.f, 0.f, 0.f};
-    // 16 bytes of channel c on of a row; behind the row's end (EVEN: whole places) anything that is there, it is not stored
-    auto take = [&](const char* row, int c) -> raw4 {
-        if constexpr (EVEN) return load16(row, min(c, width - V) * S);
-        else return c < width ? load_part((const T*)row + c, width - c) : raw4{0u, 0u, 0u, 0u};
+    // 16 bytes of channel c on at a row (uniform base, the lane's row and channel in `at`); behind the row's end (EVEN: whole
+    // places) anything that is there, it is not stored
+    auto take = [&](const char* base, uint32_t at, int c) -> raw4 {
+        if constexpr (EVEN) return load16(base, at + min(c, width - V) * S);
+        else return c < width ? load_part((const T*)(base + at) + c, width - c) : raw4{0u, 0u, 0u, 0u};
     };
+    uint32_t rank_at[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) rank_at[r] = min(r0 + 16 * r + col, p.rank - 1);
     int piece = place(rt.cum, u0);
     for (int u = u0; u < u1; ++piece) {                          // the pieces of a chunk, each a run of neighbouring tokens
         const int stop = min(u1, rt.cum[piece + 1]);
@@ -573,10 +580,12 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
                 float w[RT][8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int t = i + 8 * g + j, at = WHOLE ? t : min(t, n - 1);
-                    raw[j] = take(zp + at * ld * S, c0 + 8 * col);
+                    const int t = i + 8 * g + j;
+                    const int at = WHOLE ? i + j : min(i + j, n - 1);
+                    const uint32_t row = WHOLE ? 8 * g : max(min(8 * g, n - 1 - at), 0);
+                    raw[j] = take(zp + (int64_t)at * ld * S, row * (uint32_t)ld * S, c0 + 8 * col);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) w[r][j] = vp[at * p.rank + min(r0 + 16 * r + col, p.rank - 1)];
+                    for (int r = 0; r < RT; ++r) w[r][j] = *(const float*)((const char*)(vp + (int64_t)at * p.rank) + 4 * (row * p.rank + rank_at[r]));
                     if constexpr (!WHOLE) {
                         raw[j] = t < n ? raw[j] : zero;
 #pragma unroll
@@ -605,11 +614,12 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
                 float w[RT][4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int t = i + 4 * j + g, at = WHOLE ? t : min(t, n - 1);
+                    const int t = i + 4 * j + g, at = WHOLE ? i + 4 * j : min(i + 4 * j, n - 1);
+                    const uint32_t row = WHOLE ? g : max(min(g, n - 1 - at), 0);
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) raw[j][m] = take(zp + at * ld * S, c0 + 64 * m + 4 * col);
+                    for (int m = 0; m < 2; ++m) raw[j][m] = take(zp + (int64_t)at * ld * S, row * (uint32_t)ld * S, c0 + 64 * m + 4 * col);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) w[r][j] = vp[at * p.rank + min(r0 + 16 * r + col, p.rank - 1)];
+                    for (int r = 0; r < RT; ++r) w[r][j] = *(const float*)((const char*)(vp + (int64_t)at * p.rank) + 4 * (row * p.rank + rank_at[r]));
                     if constexpr (!WHOLE) {
 #pragma unroll
                         for (int m = 0; m < 2; ++m) raw[j][m] = t < n ? raw[j][m] : zero;
@@ -647,21 +657,49 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
             }
     }
 }
-// da, db: the chunks of an adapter in order
+// da, db: the chunks of an adapter in order.  64 channels x 16 ranks a workgroup; db's ranks leave side by side, through LDS.
 __global__ __launch_bounds__(256) void lora_reduce_kernel(ReduceTable rt, int cin, int cout, int rank, const float* part, float* da, float* db) {
-    const int c = (int)blockIdx.x * 256 + (int)threadIdx.x, r = blockIdx.y, k = blockIdx.z;
-    if (c >= cin + cout) return;
+    __shared__ float tile[64][17];
+    const int nx = (cin + 63) / 64, k = blockIdx.z, r0 = 16 * blockIdx.y;
+    const bool of_x = (int)blockIdx.x < nx;
+    const int width = of_x ? cin : cout, c = 64 * ((int)blockIdx.x - (of_x ? 0 : nx)) + ((int)threadIdx.x & 63);
     const int64_t step = (int64_t)rank * (cin + cout);
-    const float* q = part + (int64_t)rt.first[k] * step + (int64_t)r * (cin + cout) + c;
-    int n = rt.first[k + 1] - rt.first[k];
-    float s = 0.f;
-    for (; n >= 4; n -= 4, q += 4 * step) {                      // (four loads at once, added in order)
-        const float v0 = q[0], v1 = q[step], v2 = q[2 * step], v3 = q[3 * step];
-        s += v0; s += v1; s += v2; s += v3;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < width) {
+        const float* q = part + (int64_t)rt.first[k] * step + (of_x ? 0 : cin) + c;
+        int64_t row[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row[j] = (int64_t)min(r0 + ((int)threadIdx.x >> 6) + 4 * j, rank - 1) * (cin + cout);
+        int n = rt.first[k + 1] - rt.first[k];
+        for (; n >= 2; n -= 2, q += 2 * step) {                  // (eight loads at once, added in order)
+            float v[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i][j] = q[i * step + row[j]];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] += v[i][j];
+        }
+        if (n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += q[row[j]];
     }
-    for (; n > 0; --n, q += step) s += *q;
-    if (c < cin) da[((int64_t)(rt.base + k) * rank + r) * cin + c] = s;
-    else db[((int64_t)(rt.base + k) * cout + (c - cin)) * rank + r] = s;
+    if (of_x) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = r0 + ((int)threadIdx.x >> 6) + 4 * j;
+            if (c < width && r < rank) da[((int64_t)(rt.base + k) * rank + r) * cin + c] = s[j];
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tile[threadIdx.x & 63][((int)threadIdx.x >> 6) + 4 * j] = s[j];
+    __syncthreads();
+    const int r = threadIdx.x & 15, o0 = 64 * ((int)blockIdx.x - nx);
+    for (int i = threadIdx.x >> 4; i < 64; i += 16)
+        if (o0 + i < cout && r0 + r < rank) db[((int64_t)(rt.base + k) * cout + o0 + i) * rank + r0 + r] = tile[i][r];
 }
 
 template <class F> hipError_t by_rank(int rank, F&& f) {
@@ -703,10 +741,16 @@ template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::S
     });
 }
 
-// tokens of a chunk of the weight's gradient: two workgroups a CU once there are tokens for them
+// workgroups along the channels and rank shares of the weight's gradient (as lora_weight_kernel takes them apart)
+int weight_groups(const k82_lora_grad& p) {
+    const int shares = (p.rank + 31) / 32, pair = shares > 1 ? 2 : 1, per = kWaves / pair;
+    return ((p.cin + 127) / 128 + (p.cout + 127) / 128 + per - 1) / per * ((shares + pair - 1) / pair);
+}
+// Tokens of a chunk of it: two (rank > 16: three, all that fit) workgroups a CU once there are tokens for them; more would not
+// run at once and their partial sums are traffic (65536 tokens 768 / 2048 rank 16: 512 workgroups 204 us for the whole
+// backward pass, 768 213 us).
 int chunk_rows(const k82_lora_grad& p, int64_t tokens) {
-    const int64_t slices = ((p.cin + 127) / 128 + (p.cout + 127) / 128 + kWaves - 1) / kWaves;
-    const int64_t chunks = std::max<int64_t>(1, 512 / slices);
+    const int64_t chunks = std::max<int64_t>(1, (p.rank <= 16 ? 512 : 768) / weight_groups(p));
     return (int)std::max<int64_t>(32, ((tokens + chunks - 1) / chunks + 31) / 32 * 32);
 }
 struct Layout { int64_t g, at, bt, scale, part, end; };         // bytes
@@ -751,17 +795,16 @@ template <class T> hipError_t backward(const k82_lora_grad& p, const k82_segment
     const k82_lora f{p.dtype, K82_ROWS, K82_ACT_NONE, p.cout, p.cin, p.rank, (int)used.size(), p.tokens, p.dy, p.lddy,
                      p.dx_base, p.lddx_base, p.dx, p.lddx, bt, at, scale, g};
     OP_TRY(forward<T>(f, segs, st));
-    const int slices = ((p.cin + 127) / 128 + (p.cout + 127) / 128 + kWaves - 1) / kWaves;
     const bool even = p.cin % Vec<T>::N == 0 && p.cout % Vec<T>::N == 0;
     for (size_t i = 0; i < plan.tables.size(); ++i) {
         const RunTable& t = plan.tables[i];
         const auto kernel = p.rank <= 16 ? (even ? lora_weight_kernel<T, 1, true> : lora_weight_kernel<T, 1, false>)
                                          : (even ? lora_weight_kernel<T, 2, true> : lora_weight_kernel<T, 2, false>);
-        OP_TRY(op::run(kernel, dim3(slices, t.chunk0[t.runs] - t.chunk0[0], (p.rank + 31) / 32), dim3(64 * kWaves), 0, st, t, p, (const float*)g,
+        OP_TRY(op::run(kernel, dim3(weight_groups(p), t.chunk0[t.runs] - t.chunk0[0]), dim3(64 * kWaves), 0, st, t, p, (const float*)g,
                        (const float*)scale, first[i], part));
     }
     for (const ReduceTable& t : plan.reduce)
-        OP_TRY(op::run(lora_reduce_kernel, dim3((p.cin + p.cout + 255) / 256, p.rank, t.n), dim3(256), 0, st, t, p.cin, p.cout, p.rank,
+        OP_TRY(op::run(lora_reduce_kernel, dim3((p.cin + 63) / 64 + (p.cout + 63) / 64, (p.rank + 15) / 16, t.n), dim3(256), 0, st, t, p.cin, p.cout, p.rank,
                        (const float*)part, p.da, p.db));
     return hipSuccess;
 }
