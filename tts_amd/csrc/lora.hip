@@ -167,7 +167,7 @@ constexpr int kPad = 4;                        // floats behind a row of the res
 // (waves_per_eu: without it the accumulators of four and eight rank tiles are copied through the second register file and one
 // wave less fits a SIMD; 65536 tokens 2048 -> 768 bf16 rank 64: 146 us, with it 137.)
 template <class T, int NW, int RT, int TT, bool EVEN>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8 ? 2 : RT >= 4 ? 3 : 4))) void lora_rows_kernel(SegTable sg, k82_lora p) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8 ? 1 : RT >= 4 ? 3 : 4))) void lora_rows_kernel(SegTable sg, k82_lora p) {
     constexpr int V = Vec<T>::N, K = 4 * V, S = sizeof(T), U = RT + TT > 4 ? 2 : 4;          // U: steps whose loads are in flight together
     constexpr int CH = 8 * V, MT = CH / 16, CK = Second<T, RT>::CHUNKS;          // channels, row tiles of B, chunks of a row of B
     constexpr int kTiles = most(RT + TT, MT * CK), kRow = CH + kPad;
@@ -336,8 +336,9 @@ template <int TT> __device__ __forceinline__ void load_tokens(float (&v)[TT], co
         v[1] = r[1];
     } else v[0] = *(const float*)(base + at);
 }
+// (waves_per_eu as above: 65536 x 768 rank 32 192 us, with it 165.)
 template <int NW, int RT, int TT, bool EVEN>
-__global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lora p) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8 ? 2 : RT >= 4 ? 3 : 4))) void lora_cols_kernel(SegTable sg, k82_lora p) {
     constexpr int U = 2;
     __shared__ __align__(16) char lds[most(NW * RT * 1024, NW * RT * TT * 1024)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
@@ -346,6 +347,15 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
     const int tile = first / (16 * TT) * (16 * TT) + (int)blockIdx.x * 16 * TT, t0 = tile + TT * col;
     const uint32_t tb = 4 * min(t0, tokens - TT);
     const bool second = t0 == tokens - 1;
+    // the lane's four channels (4 g + i) of 16 from base on, n of them there; behind those any that is (EVEN: four at a time, so
+    // that one register holds the lane's offset)
+    auto load_rows = [&](float (&v)[4][TT], const char* base, int64_t ld, int n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (EVEN) load_tokens<TT>(v[i], base + i * ld * 4, min(4 * g, n - 4) * (uint32_t)ld * 4 + tb, second);
+            else load_tokens<TT>(v[i], base, min(4 * g + i, n - 1) * (uint32_t)ld * 4 + tb, second);
+        }
+    };
     int s = place(sg.tile0, max(tile, first) - first);
     for (; s < sg.n && sg.start[s] < tile + 16 * TT; ++s) {
         const int k = sg.index[s], lo = sg.start[s], hi = lo + sg.len[s];
@@ -359,8 +369,7 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
             const int n = p.cout - 16 * blk;
             if (p.base) {
                 const char* q = (const char*)p.base + (int64_t)16 * blk * p.ldbase * 4;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) load_tokens<TT>(base[i], q, min(4 * g + i, n - 1) * (uint32_t)p.ldbase * 4 + tb, second);
+                load_rows(base, q, p.ldbase, n);
             }
             if (k >= 0) {
                 const uint32_t at = (min(lane >> 2, n - 1) * (uint32_t)p.rank + c4) * 4;
@@ -408,7 +417,7 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
                     const int c0 = 16 * (i0 + u * NW);
                     const char* q = (const char*)p.x + (int64_t)c0 * p.ldx * 4;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) load_tokens<TT>(fx[u][i], q, (4 * g + i) * (uint32_t)p.ldx * 4 + tb, second);
+                    for (int i = 0; i < 4; ++i) load_tokens<TT>(fx[u][i], q + (int64_t)i * p.ldx * 4, 4 * g * (uint32_t)p.ldx * 4 + tb, second);
 #pragma unroll
                     for (int r = 0; r < RT; ++r) fa[u][r] = load16(ap + 4 * c0, ao[r]);
                 }
@@ -426,12 +435,11 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
                 float fx[4][TT];
 #pragma unroll
                 for (int r = 0; r < RT; ++r) fa[r] = grab<float, EVEN>(ap + 4 * c0, ao[r], n - c4, 4 * c4);
+                load_rows(fx, q, p.ldx, n);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    load_tokens<TT>(fx[i], q, min(4 * g + i, n - 1) * (uint32_t)p.ldx * 4 + tb, second);
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int t = 0; t < TT; ++t) fx[i][t] = 4 * g + i < n ? fx[i][t] : 0.f;
-                }
                 multiply(fa, fx);
             }
             int64_t tok[TT];
@@ -468,7 +476,7 @@ __global__ __launch_bounds__(64 * NW) void lora_cols_kernel(SegTable sg, k82_lor
 #pragma unroll
                 for (int t = 0; t < TT; ++t) v[t] = p.act == K82_ACT_GELU_NEW ? op_gelu_new(d[t][i]) : d[t][i];
                 if (16 * blk + c >= p.cout) continue;
-                float* q = (float*)(yb + (c * (uint32_t)p.ldy + t0) * 4);
+                float* q = (float*)(yb + (int64_t)i * p.ldy * 4 + (4 * g * (uint32_t)p.ldy + t0) * 4);
                 if (t0 >= lo && t0 + TT <= hi) {
                     if constexpr (TT == 2) *(f2_any*)q = f2_any{v[0], v[1]};
                     else q[0] = v[0];
