@@ -93,7 +93,7 @@ int k82_destroy(k82_handle* h);
  * replaces: the reference's two worker threads on one Kokoro object (epubviewer_06_latest_1_nov_2025_theme.py:407,692,715),
  * which onnxruntime serves with concurrent sess.run calls on one InferenceSession. */
 int k82_fork(k82_handle* parent, k82_handle** out);
-const char* k82_last_error(const k82_handle* h); /* h may be NULL: last create error */
+const char* k82_last_error(const k82_handle* h); /* h may be NULL: this thread's last error of a call without a handle (create, checks) */
 
 /* Weight upload.  `name` is "<submodule>.<state-dict key>" with weight-norm already folded
  * (e.g. "decoder.generator.ups.0.weight"), data is host f32 in PyTorch layout.  The layer
@@ -223,8 +223,10 @@ int k82_pcm16_static(k82_handle* h, const float* src, int16_t* dst, int64_t n, v
  * needed.  At most 2^24 - 1 tokens, 2^20 channels and an ld of 2^25 a call.
  *
  * Segments cut the token axis: segment s holds the tokens [off[s], off[s+1]), 0 <= off[0] <= ... <= off[n] <= tokens,
- * and uses adapter (gain) index[s]; an index may come any number of times and a segment may be empty.  Output rows that
- * no segment holds are left as they were. */
+ * and uses adapter (gain) index[s]; an index may come any number of times and a segment may be empty.  K82_SKIP (the padding
+ * of a padded batch): its tokens belong to nobody.  Output rows that no segment holds, or a skipped one, are left as they
+ * were, and what lies in the inputs there reaches no result. */
+#define K82_SKIP (-2)
 #define K82_F32 0
 #define K82_BF16 1
 #define K82_ROWS 0
@@ -239,7 +241,7 @@ typedef struct k82_segments {
     int32_t n;            /* >= 0 */
 } k82_segments;
 
-/* y = act(base + scale[k] * (x A_k^T) B_k^T), k = index of the token's segment; k = -1: y = act(base).
+/* y = act(base + scale[k] * (x A_k^T) B_k^T), k = index of the token's segment; k = -1 (no adapter): y = act(base).
  * base is what the shared projection wrote (NULL: 0) and may be y itself; x and y must not overlap.  Products of 16-bit
  * operands are exact, all sums are 32 bits wide, and y is rounded once.
  * h (NULL: not kept): f32[tokens][rank], x A_k^T (0 where k = -1), which k82_op_lora_grad takes. */
@@ -285,7 +287,7 @@ int k82_op_lora_grad(k82_handle* h, const k82_lora_grad* p, const k82_segments* 
 int64_t k82_op_lora_grad_workspace(const k82_lora_grad* p, const k82_segments* seg);
 
 /* z = x + res (res NULL: z = x); y = (z - mean) * rstd * gain_k + offset_k over the channels of a token,
- * rstd = 1 / sqrt(var + eps), var the mean square around the mean.  0 <= k < gains.  y may be x or res itself.
+ * rstd = 1 / sqrt(var + eps), var the mean square around the mean.  0 <= k < gains (or K82_SKIP).  y may be x or res itself.
  * mean, rstd (both or neither): f32[tokens], which k82_op_layernorm_grad takes. */
 typedef struct k82_layernorm {
     int32_t dtype, layout;

@@ -73,7 +73,9 @@ def test_ordinary_arguments_are_accepted(which):
     ("lora", dict(base=6 * P, ldbase=23), "ld of base"), ("lora", dict(x=P + 2), "aligned"),
     ("lora", dict(y=P), "overlap"), ("lora", dict(y=P + 8 * 4), "overlap"), ("lora", dict(base=2 * P + 4, ldbase=24), "overlap"),
     ("lora", dict(base=2 * P, ldbase=25, ldy=24), "overlap"), ("lora", dict(h=2 * P), "overlaps"),
-    ("lora", dict(layout=1, ldx=9, ldy=10), "ld of x"),
+    ("lora", dict(layout=1, ldx=9, ldy=10), "ld of x"), ("lora", dict(ldx=(1 << 25) + 1), "2^25"), ("lora", dict(a=3 * P + 1), "aligned"),
+    ("lora", dict(h=9 * P + 2), "aligned"), ("lora_grad", dict(da=8 * P + 1), "aligned"), ("norm", dict(gain=3 * P + 2), "aligned"),
+    ("norm_grad", dict(rstd=6 * P + 1), "aligned"), ("lora", dict(tokens=1 << 24), "tokens"),
     ("lora_grad", dict(dtype=3), "dtype"), ("lora_grad", dict(rank=200), "rank"), ("lora_grad", dict(h=None), "h must not"),
     ("lora_grad", dict(da=None), "da and db"), ("lora_grad", dict(dx=P), "overlaps"), ("lora_grad", dict(dx=2 * P), "overlaps"),
     ("lora_grad", dict(dx_base=4 * P + 4, lddx_base=16), "without being one"), ("lora_grad", dict(lddy=23), "ld of dy"),
@@ -92,7 +94,7 @@ def test_bad_arguments_are_refused(which, kw, word):
 @pytest.mark.parametrize("which", FUNCTIONS)
 @pytest.mark.parametrize("off,index,word", [
     ([0, 5, 4], [0, 1], "decrease"), ([-1, 4, 10], [0, 1], "negative"), ([0, 4, 11], [0, 1], "10 tokens"),
-    ([0, 4, 10], [0, 2], "index 2"), ([0, 4, 10], [-2, 1], "index -2"),
+    ([0, 4, 10], [0, 2], "index 2"), ([0, 4, 10], [-3, 1], "index -3"),
 ])
 def test_bad_segments_are_refused(which, off, index, word):
     rc, msg = answer(which, raw_segments(off, index))
@@ -137,8 +139,27 @@ def test_segments_class_refuses_what_is_not_a_cut():
     for off, index in (([0, 2], [0, 1]), ([0, 3, 2], [0, 1]), ([-1, 3], [0]), ([[0, 1]], [0])):
         with pytest.raises(ValueError):
             Segments(off, index)
+    for off, index, word in (([0.0, 2.5], [0], "whole numbers"), ([0, 2], [0.5], "whole numbers"), ([0, 2], [1 << 32], "32 bits")):
+        with pytest.raises(ValueError, match=word):
+            Segments(off, index)
     with pytest.raises(ValueError):
         s.offsets[0] = 5                                        # the library reads this memory
+    mine = np.array([0, 4], np.int64)
+    s = Segments(mine, np.array([0], np.int32))
+    mine[1] = 99
+    assert s.offsets.tolist() == [0, 4]
+
+
+def test_padded_batches_are_cut_into_sentences_and_padding():
+    s = Segments.of_padded([3, 0, 5], [1, 0, -1], 5)
+    assert s.offsets.tolist() == [0, 3, 5, 5, 10, 15, 15] and s.index.tolist() == [1, -2, 0, -2, -1, -2]
+    assert not s.covers(15) and Segments([0, 15], [0]).covers(15) and not Segments([0, 14], [0]).covers(15)
+    for which in FUNCTIONS:
+        rc, msg = answer(which, raw_segments([0, 3, 5, 10], [1, -2, 0]))
+        assert rc >= 0, msg
+    for lengths, index in (([6], [0]), ([-1], [0]), ([1, 2], [0])):
+        with pytest.raises(ValueError):
+            Segments.of_padded(lengths, index, 5)
 
 
 def test_python_face_refuses_before_the_library():

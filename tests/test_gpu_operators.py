@@ -497,6 +497,52 @@ def _norm64(x, res, gain, offset, seg):
     return torch.cat([xh[lo:hi] * gain[k] + offset[k] for lo, hi, k in spans(seg)])
 
 
+# ---------------------------------------------------------------------------------------------- padded batches
+@pytest.mark.parametrize("dt,kind", [(torch.float32, "dense"), (torch.float32, "cols"), (torch.bfloat16, "dense")])
+@pytest.mark.parametrize("pitch,lengths", [(40, [13, 40, 0, 1, 33]), (7, [3] * 150), (64, [64, 64, 5])])
+def test_padding_is_left_alone_and_reaches_nothing(ops, dt, kind, pitch, lengths):
+    n, c = len(lengths), 72
+    tokens = n * pitch
+    index = [i % 3 for i in range(n)]
+    padded, packed = Segments.of_padded(lengths, index, pitch), Segments.of_lengths(lengths, index)
+    rows = torch.cat([torch.arange(b * pitch, b * pitch + m) for b, m in enumerate(lengths)]).cuda()
+    pad = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    pad[rows] = False
+    x, base, a, b, scale = lora_case(tokens, c, c, 6, 3, dt, kind, 81)
+    gain, offset = (1 + 0.1 * gen(82)(3, c)).to(dt), gen(83)(3, c).to(dt)
+    x[pad], base[pad] = float("nan"), float("inf")
+
+    def pack(t):
+        v = t[rows].contiguous()
+        return v.t().contiguous().t() if kind == "cols" else v
+
+    def same(got, want):
+        assert torch.equal(got[rows], want)
+        assert (got[pad] == 0).all()                             # (outputs of the call's own making)
+
+    y, h = ops.op_lora(x, a, b, scale, padded, base=base, keep=True)
+    yp, hp = ops.op_lora(pack(x), a, b, scale, packed, base=pack(base), keep=True)
+    same(y, yp)
+    same(h, hp)
+    out = torch.full_like(x, SENTINEL)
+    z, mean, rstd = ops.op_layernorm(x, gain, offset, padded, res=base, out=out, stats=True)
+    zp, mp, rp = ops.op_layernorm(pack(x), gain, offset, packed, res=pack(base), stats=True)
+    assert torch.equal(z[rows], zp) and (out[pad] == SENTINEL).all()
+    same(mean, mp)
+    same(rstd, rp)
+    if kind == "cols":
+        return
+    mean[pad], rstd[pad], h[pad] = float("nan"), float("inf"), float("nan")
+    got = ops.op_layernorm_grad(x, base, gain, mean, rstd, padded)
+    same(got[0], ops.op_layernorm_grad(pack(x), pack(base), gain, mp, rp, packed)[0])
+    for g, (w, bound) in zip(got[1:], norm_grad_want(pack(x), None, pack(base), gain, mp, rp, packed)[1:]):
+        within(g, w, bound, "gain")
+    got = ops.op_lora_grad(x, base, h, a, b, scale, padded)
+    same(got[0], ops.op_lora_grad(pack(x), pack(base), hp, a, b, scale, packed)[0])
+    for g, (w, bound) in zip(got[1:], lora_grad_want(pack(x), pack(base), hp, None, a, b, scale, packed)[1:]):
+        within(g, w, bound + 1e-38, "factors")
+
+
 # ---------------------------------------------------------------------------------------------- as they are used
 def sublayer(ops, x, w, a, b, scale, gain, offset, seg, eps=1e-5):
     """A projection with adapters, the residual and the norm: forward."""

@@ -359,6 +359,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
     int s = place(sg.tile0, max(tile, first) - first);
     for (; s < sg.n && sg.start[s] < tile + 16 * TT; ++s) {
         const int k = sg.index[s], lo = sg.start[s], hi = lo + sg.len[s];
+        if (k == K82_SKIP) continue;
         if (k < 0 && p.act == K82_ACT_NONE && p.base == p.y && !p.h) continue;
         const int blocks = (p.cout + 15) / 16, stride = NW * gridDim.y;
         int blk = (int)blockIdx.y * NW + wave;
@@ -821,7 +822,8 @@ template <class T> hipError_t backward(const k82_lora_grad& p, const k82_segment
 namespace op {
 int64_t workspace(const k82_lora_grad& p, const k82_segments& s) { return layout(p, s).end; }
 hipError_t launch(const k82_lora& p, const k82_segments& s, hipStream_t st) {
-    return p.dtype == K82_F32 ? forward<float>(p, merged(s), st) : forward<bf16_t>(p, merged(s), st);
+    const std::vector<Seg> segs = merged(s, p.layout == K82_COLS);
+    return p.dtype == K82_F32 ? forward<float>(p, segs, st) : forward<bf16_t>(p, segs, st);
 }
 hipError_t launch(const k82_lora_grad& p, const k82_segments& s, void* ws, hipStream_t st) {
     return p.dtype == K82_F32 ? backward<float>(p, s, ws, st) : backward<bf16_t>(p, s, ws, st);

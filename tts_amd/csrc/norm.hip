@@ -34,12 +34,23 @@ __global__ __launch_bounds__(kThreads<W>) void norm_rows_kernel(SegTable sg, k82
     __shared__ float sh[2][W];
     const int lane = W == 1 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
     const int wave = W == 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0;
-    const int first = sg.start[0], end = first + min((int)sg.tile0[sg.n], ((int)blockIdx.x + 1) * tile);
-    int t = first + (int)blockIdx.x * tile + wave, seg_end = t;
+    const int seg = seg_of(sg, blockIdx.x), begin = ((int)blockIdx.x - sg.tile0[seg]) * tile;
+    const int end = sg.start[seg] + min(sg.len[seg], begin + tile);
+    int t = sg.start[seg] + begin + wave;
     float g[NV][N], o[NV][N];
     int left[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) left[i] = p.c - (lane + i * 64 * W) * N;       // channels from this vector on
+    for (int i = 0; i < NV; ++i) {
+        const int c = (lane + i * 64 * W) * N;
+        left[i] = p.c - c;                                       // channels from this vector on
+        raw4 a = {0u, 0u, 0u, 0u}, b = a;
+        if (left[i] > 0) {
+            a = load_part((const T*)p.gain + (int64_t)sg.index[seg] * p.c + c, left[i]);
+            b = load_part((const T*)p.offset + (int64_t)sg.index[seg] * p.c + c, left[i]);
+        }
+        Vec<T>::unpack(a, g[i]);
+        Vec<T>::unpack(b, o[i]);
+    }
     auto fetch = [&](int64_t row, raw4* rx, raw4* rr) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -66,19 +77,6 @@ __global__ __launch_bounds__(kThreads<W>) void norm_rows_kernel(SegTable sg, k82
             for (int j = 0; j < N; ++j) { z[i][j] += r[j]; s += z[i][j]; }
         }
         if (t + R < end) fetch(t + R, rx, rr);                   // the next row is on its way while this one is summed
-        if (t >= seg_end) {                                      // (uniform) another sentence: its gain and offset
-            const int i = seg_of(sg, t - first);
-            seg_end = first + sg.tile0[i + 1];
-            const T *gp = (const T*)p.gain + (int64_t)sg.index[i] * p.c, *op = (const T*)p.offset + (int64_t)sg.index[i] * p.c;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int c = (lane + v * 64 * W) * N;
-                raw4 a = {0u, 0u, 0u, 0u}, b = a;
-                if (left[v] > 0) { a = load_part(gp + c, left[v]); b = load_part(op + c, left[v]); }
-                Vec<T>::unpack(a, g[v]);
-                Vec<T>::unpack(b, o[v]);
-            }
-        }
         const float mean = row_total<W>(s, sh[0]) / p.c;
         float q = 0.f;
 #pragma unroll
@@ -119,7 +117,7 @@ template <int Q, int NW, int NV> __global__ __launch_bounds__(64 * NW) void norm
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quad = lane & (Q - 1);
     const int first = sg.start[0], end = first + sg.tile0[sg.n];
     const int t0 = (first & ~(TOK - 1)) + (int)blockIdx.x * TOK + 4 * quad, c0 = 64 / Q * wave + lane / Q;
-    const bool whole = t0 >= first && t0 + 4 <= end;
+    const bool whole = t0 >= first && t0 + 4 <= end;             // (what is loaded there; skipped tokens are not stored)
     if (threadIdx.x < TOK) {
         const int t = min(max((first & ~(TOK - 1)) + (int)blockIdx.x * TOK + (int)threadIdx.x, first), end - 1) - first;
         int s = 0;
@@ -176,29 +174,32 @@ template <int Q, int NW, int NV> __global__ __launch_bounds__(64 * NW) void norm
     q = total(q, red[1]);
     const float4 rstd = make_float4(1.0f / sqrtf(q.x / p.c + p.eps), 1.0f / sqrtf(q.y / p.c + p.eps),
                                     1.0f / sqrtf(q.z / p.c + p.eps), 1.0f / sqrtf(q.w / p.c + p.eps));
+    const int k0 = kind[4 * quad], k1 = kind[4 * quad + 1], k2 = kind[4 * quad + 2], k3 = kind[4 * quad + 3];
+    const bool stored[4] = {t0 >= first && t0 < end && k0 >= 0, t0 + 1 >= first && t0 + 1 < end && k1 >= 0,
+                            t0 + 2 >= first && t0 + 2 < end && k2 >= 0, t0 + 3 >= first && t0 + 3 < end && k3 >= 0};
+    const bool all4 = stored[0] && stored[1] && stored[2] && stored[3];
     auto store = [&](float* v, float4 y) {
-        if (whole) { *(raw4_f*)v = raw4{__float_as_uint(y.x), __float_as_uint(y.y), __float_as_uint(y.z), __float_as_uint(y.w)}; return; }
+        if (all4) { *(raw4_f*)v = raw4{__float_as_uint(y.x), __float_as_uint(y.y), __float_as_uint(y.z), __float_as_uint(y.w)}; return; }
         const float a[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (t0 + j >= first && t0 + j < end) v[j] = a[j];
+            if (stored[j]) v[j] = a[j];
     };
     if (p.mean && c0 == 0) { store(p.mean + t0, mean); store(p.rstd + t0, rstd); }
     const float *gain = (const float*)p.gain, *offset = (const float*)p.offset;
-    const int k0 = kind[4 * quad], k1 = kind[4 * quad + 1], k2 = kind[4 * quad + 2], k3 = kind[4 * quad + 3];
     const bool uniform = __all(k0 == kind[0] && k1 == kind[0] && k2 == kind[0] && k3 == kind[0]);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = c0 + STEP * i;
         if (c >= p.c) continue;
         float4 g, o;
-        const int64_t at = (int64_t)k0 * p.c + c;
+        const int64_t at = (int64_t)max(k0, 0) * p.c + c;
         g.x = gain[at]; o.x = offset[at];
         if (uniform) {
             g = make_float4(g.x, g.x, g.x, g.x);
             o = make_float4(o.x, o.x, o.x, o.x);
         } else {
-            const int64_t a1 = (int64_t)k1 * p.c + c, a2 = (int64_t)k2 * p.c + c, a3 = (int64_t)k3 * p.c + c;
+            const int64_t a1 = (int64_t)max(k1, 0) * p.c + c, a2 = (int64_t)max(k2, 0) * p.c + c, a3 = (int64_t)max(k3, 0) * p.c + c;
             g = make_float4(g.x, gain[a1], gain[a2], gain[a3]);
             o = make_float4(o.x, offset[a1], offset[a2], offset[a3]);
         }
@@ -414,33 +415,36 @@ template <class T, int MAX, class F> hipError_t by_width(int c, F&& f) {
 
 template <class T> hipError_t forward(const k82_layernorm& p, const k82_segments& s, hipStream_t st) {
     const bool cols = p.layout == K82_COLS;
-    for (const SegTable& t : op::tables(op::merged(s), 1)) {
-        const int tokens = t.tile0[t.n];
-        if (cols && p.c <= kColsMax) {
+    if (cols && p.c <= kColsMax) {
+        for (const SegTable& t : op::tables(op::merged(s, true), 1)) {
+            const int tokens = t.tile0[t.n];
             auto go = [&](auto q, auto w, auto v) {
                 constexpr int Q = decltype(q)::value, NW = decltype(w)::value;
                 const int tiles = (t.start[0] + tokens - 1) / (4 * Q) - t.start[0] / (4 * Q) + 1;
                 return op::run(norm_cols_kernel<Q, NW, decltype(v)::value>, dim3(tiles), dim3(64 * NW), 0, st, t, p);
             };
-            const std::integral_constant<int, 12> v12; const std::integral_constant<int, 2> q2; const std::integral_constant<int, 4> q4; const std::integral_constant<int, 8> q8;
-            const std::integral_constant<int, 16> w16;
+            const std::integral_constant<int, 12> v12; const std::integral_constant<int, 2> q2; const std::integral_constant<int, 4> q4;
+            const std::integral_constant<int, 8> q8; const std::integral_constant<int, 16> w16;
             OP_TRY(p.c <= 256 ? go(q8, q8, q4) : p.c <= 512 ? go(q8, q8, q8) : p.c <= 768 ? go(q8, q8, v12) :
                    p.c <= 1536 ? go(q8, w16, v12) : p.c <= 2048 ? go(q4, w16, q8) : go(q2, w16, q8));
-            continue;
         }
-        if (cols || p.c > kRowMax) {
-            OP_TRY(op::run(norm_token_kernel<T>, dim3(tokens), dim3(256), 0, st, t, p, cols ? 1 : p.ldx, cols ? p.ldx : 1,
-                           cols ? 1 : p.ldres, cols ? p.ldres : 1, cols ? 1 : p.ldy, cols ? p.ldy : 1));
-            continue;
-        }
-        OP_TRY(by_width<T, kRowMax>(p.c, [&](auto w, auto nv) {
-            constexpr int W = decltype(w)::value, R = W == 1 ? 4 : 1;
-            // rows behind each other in a workgroup share the gain's registers, once there are rows for every CU
-            const int tile = R * std::max(1, std::min(4, tokens / (R * 2048)));
-            return op::run(norm_rows_kernel<T, W, decltype(nv)::value>, dim3((tokens + tile - 1) / tile), dim3(kThreads<W>), 0, st, t, p, tile);
-        }));
+        return hipSuccess;
     }
-    return hipSuccess;
+    const std::vector<op::Seg> segs = op::merged(s);
+    if (cols || p.c > kRowMax) {
+        for (const SegTable& t : op::tables(segs, 1))
+            OP_TRY(op::run(norm_token_kernel<T>, dim3(t.tile0[t.n]), dim3(256), 0, st, t, p, cols ? 1 : p.ldx, cols ? p.ldx : 1,
+                           cols ? 1 : p.ldres, cols ? p.ldres : 1, cols ? 1 : p.ldy, cols ? p.ldy : 1));
+        return hipSuccess;
+    }
+    return by_width<T, kRowMax>(p.c, [&](auto w, auto nv) -> hipError_t {
+        constexpr int W = decltype(w)::value, R = W == 1 ? 4 : 1;
+        // rows behind each other in a workgroup share the gain's registers, once there are rows for every CU
+        const int tile = R * (int)std::max<int64_t>(1, std::min<int64_t>(4, op::covered(s) / (R * 2048)));
+        for (const SegTable& t : op::tables(segs, tile))
+            OP_TRY(op::run(norm_rows_kernel<T, W, decltype(nv)::value>, dim3(t.tile0[t.n]), dim3(kThreads<W>), 0, st, t, p, tile));
+        return hipSuccess;
+    });
 }
 
 // Tokens of a chunk: one workgroup for every place on the 256 CUs once there are tokens for them (the registers leave

@@ -22,7 +22,8 @@ struct SegTable {
 };
 struct Seg { int start, len, index; };
 
-std::vector<Seg> merged(const k82_segments& s);
+// without the skipped segments, or (walked) with those between others: kernels that walk the token axis pass over them
+std::vector<Seg> merged(const k82_segments& s, bool walked = false);
 // tables of at most kSegs segments with `tile` tokens per tile
 std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile);
 

@@ -34,7 +34,7 @@ std::string check_segments(const k82_segments* s, int64_t tokens, int lo, int hi
     if (s->off[0] < 0) return "segments: off[0] must not be negative";
     for (int32_t i = 0; i < s->n; ++i) {
         if (s->off[i + 1] < s->off[i]) return "segments: off must not decrease (at " + std::to_string(i) + ")";
-        if (s->index[i] < lo || s->index[i] >= hi)
+        if ((s->index[i] < lo && s->index[i] != K82_SKIP) || s->index[i] >= hi)
             return std::string("segments: index ") + std::to_string(s->index[i]) + " of segment " + std::to_string(i) +
                    " is outside [" + std::to_string(lo) + ", " + what + " = " + std::to_string(hi) + ")";
     }
@@ -57,6 +57,11 @@ std::string check_tensor(const char* name, const void* p, int64_t ld, int layout
     if ((uintptr_t)p % size) return std::string(name) + " is not aligned to its element";
     if (ld < (layout == K82_COLS ? tokens : c)) return std::string("ld of ") + name + " is smaller than a row of it";
     if (ld > 1 << 25) return std::string("ld of ") + name + " is larger than 2^25";       // (offsets inside a tile of 32 rows are 32 bits wide)
+    return "";
+}
+std::string check_aligned(int size, std::initializer_list<const void*> p) {
+    for (const void* v : p)
+        if ((uintptr_t)v % size) return "a pointer is not aligned to its element";
     return "";
 }
 std::string check_lora_factors(int rank, int adapters, const void* a, const void* b, const float* scale) {
@@ -83,6 +88,8 @@ std::string check(const k82_lora* p, const k82_segments* s) {
     OP_CHECK(check_tensor("x", p->x, p->ldx, p->layout, p->tokens, p->cin, size, false));
     OP_CHECK(check_tensor("base", p->base, p->ldbase, p->layout, p->tokens, p->cout, size, true));
     OP_CHECK(check_tensor("y", p->y, p->ldy, p->layout, p->tokens, p->cout, size, false));
+    OP_CHECK(check_aligned(size, {p->a, p->b}));
+    OP_CHECK(check_aligned(4, {p->scale, p->h}));
     const Span x(p->x, p->ldx, p->layout, p->tokens, p->cin, size), y(p->y, p->ldy, p->layout, p->tokens, p->cout, size),
         base(p->base, p->ldbase, p->layout, p->tokens, p->cout, size), h(p->h, p->rank, K82_ROWS, p->tokens, p->rank, 4);
     if (overlap(x, y)) return "x and y overlap";
@@ -102,6 +109,8 @@ std::string check(const k82_lora_grad* p, const k82_segments* s) {
     OP_CHECK(check_tensor("h", p->h, p->rank, K82_ROWS, p->tokens, p->rank, 4, false));
     OP_CHECK(check_tensor("dx_base", p->dx_base, p->lddx_base, K82_ROWS, p->tokens, p->cin, size, true));
     OP_CHECK(check_tensor("dx", p->dx, p->lddx, K82_ROWS, p->tokens, p->cin, size, false));
+    OP_CHECK(check_aligned(size, {p->a, p->b}));
+    OP_CHECK(check_aligned(4, {p->scale, p->h, p->da, p->db}));
     const Span x(p->x, p->ldx, K82_ROWS, p->tokens, p->cin, size), dx(p->dx, p->lddx, K82_ROWS, p->tokens, p->cin, size),
         dy(p->dy, p->lddy, K82_ROWS, p->tokens, p->cout, size), h(p->h, p->rank, K82_ROWS, p->tokens, p->rank, 4),
         base(p->dx_base, p->lddx_base, K82_ROWS, p->tokens, p->cin, size);
@@ -120,6 +129,8 @@ std::string check(const k82_layernorm* p, const k82_segments* s) {
     OP_CHECK(check_tensor("x", p->x, p->ldx, p->layout, p->tokens, p->c, size, false));
     OP_CHECK(check_tensor("res", p->res, p->ldres, p->layout, p->tokens, p->c, size, true));
     OP_CHECK(check_tensor("y", p->y, p->ldy, p->layout, p->tokens, p->c, size, false));
+    OP_CHECK(check_aligned(size, {p->gain, p->offset}));
+    OP_CHECK(check_aligned(4, {p->mean, p->rstd}));
     const Span x(p->x, p->ldx, p->layout, p->tokens, p->c, size), res(p->res, p->ldres, p->layout, p->tokens, p->c, size),
         y(p->y, p->ldy, p->layout, p->tokens, p->c, size), m(p->mean, 1, K82_ROWS, p->tokens, 1, 4), r(p->rstd, 1, K82_ROWS, p->tokens, 1, 4);
     if (overlap(x, y) && !same(x, y)) return "x and y overlap without being one tensor";
@@ -139,6 +150,8 @@ std::string check(const k82_layernorm_grad* p, const k82_segments* s) {
     OP_CHECK(check_tensor("res", p->res, p->ldres, K82_ROWS, p->tokens, p->c, size, true));
     OP_CHECK(check_tensor("dy", p->dy, p->lddy, K82_ROWS, p->tokens, p->c, size, false));
     OP_CHECK(check_tensor("dx", p->dx, p->lddx, K82_ROWS, p->tokens, p->c, size, false));
+    OP_CHECK(check_aligned(size, {p->gain}));
+    OP_CHECK(check_aligned(4, {p->mean, p->rstd, p->dgain, p->doffset}));
     const Span dx(p->dx, p->lddx, K82_ROWS, p->tokens, p->c, size);
     const Span in[3] = {{p->x, p->ldx, K82_ROWS, p->tokens, p->c, size}, {p->res, p->ldres, K82_ROWS, p->tokens, p->c, size},
                         {p->dy, p->lddy, K82_ROWS, p->tokens, p->c, size}};
@@ -150,14 +163,15 @@ std::string check(const k82_layernorm_grad* p, const k82_segments* s) {
     return "";
 }
 
-std::vector<Seg> merged(const k82_segments& s) {
+std::vector<Seg> merged(const k82_segments& s, bool walked) {
     std::vector<Seg> v;
     for (int32_t i = 0; i < s.n; ++i) {
         const int start = (int)s.off[i], len = (int)(s.off[i + 1] - s.off[i]);
-        if (len == 0) continue;
-        if (!v.empty() && v.back().index == s.index[i]) v.back().len += len;     // (neighbours: nothing lies between them)
+        if (len == 0 || (s.index[i] == K82_SKIP && (!walked || v.empty()))) continue;
+        if (!v.empty() && v.back().index == s.index[i] && v.back().start + v.back().len == start) v.back().len += len;
         else v.push_back({start, len, s.index[i]});
     }
+    while (!v.empty() && v.back().index == K82_SKIP) v.pop_back();
     return v;
 }
 std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile) {

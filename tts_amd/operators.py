@@ -3,7 +3,7 @@
 ``Operators`` is a handle without model weights; ``Engine`` is one with them and has the same methods.  Tensors are torch
 tensors on the handle's GPU -- the buffers, nothing else: every number is computed in libk82.so.  A call enqueues on
 torch's current stream and returns at once; outputs and workspaces come from torch's allocator, so a call may be captured
-into a graph.  Refused arguments raise ``ValueError`` / ``TypeError`` before anything is enqueued.
+into a graph.  There is no autograd: gradients are calls of their own (``op_*_grad``).  Refused arguments raise ``ValueError`` / ``TypeError`` before anything is enqueued.
 
 Tensors are ``[tokens, channels]``, rows (unit stride along the channels) or, float32 forward only, channel-first (unit
 stride along the tokens: ``buffer[channels, pitch].t()``, the engine's own layout).
@@ -39,25 +39,47 @@ def _cfg_struct(config):
 
 class Segments:
     """The cut of a packed token axis: segment ``s`` holds the tokens ``offsets[s]:offsets[s + 1]`` and uses adapter (or
-    gain) ``index[s]``; -1 is a sentence without an adapter.  Host data; keep it for as many calls as the batch makes."""
+    gain) ``index[s]``; -1 is a sentence without an adapter, ``Segments.SKIP`` tokens that belong to nobody (padding).  Host
+    data; keep it for as many calls as the batch makes."""
 
-    __slots__ = ("offsets", "index", "c", "address", "lo", "hi")
+    SKIP = -2
+    __slots__ = ("offsets", "index", "c", "address", "lo", "hi", "whole")
 
     def __init__(self, offsets, index):
-        self.offsets = np.array(offsets, dtype=np.int64)
-        self.index = np.array(index, dtype=np.int32)
+        offsets, index = np.asarray(offsets), np.asarray(index)
+        if (offsets.size and offsets.dtype.kind not in "iu") or (index.size and index.dtype.kind not in "iu"):
+            raise ValueError("Segments: offsets and index are whole numbers")
+        if index.size and (index.min() < -(1 << 31) or index.max() >= 1 << 31):
+            raise ValueError("Segments: an index does not fit 32 bits")
+        self.offsets = offsets.astype(np.int64)                  # copies: nobody else writes what the library reads
+        self.index = index.astype(np.int32)
         if self.offsets.ndim != 1 or self.index.ndim != 1 or self.offsets.size != self.index.size + 1:
             raise ValueError("Segments: offsets holds one value more than index")
         if self.offsets[0] < 0 or (self.offsets[1:] < self.offsets[:-1]).any():
             raise ValueError("Segments: offsets must not be negative and must not decrease")
         self.offsets.flags.writeable = self.index.flags.writeable = False
         self.lo, self.hi = int(self.offsets[0]), int(self.offsets[-1])
+        self.whole = not (self.index == self.SKIP).any()         # every token from lo to hi is somebody's
         self.c = _lib.K82Segments(off=self.offsets.ctypes.data, index=self.index.ctypes.data, n=self.index.size)
         self.address = C.addressof(self.c)
 
     @classmethod
     def of_lengths(cls, lengths, index):
-        return cls(np.concatenate([[0], np.cumsum(np.asarray(lengths, dtype=np.int64))]), index)
+        return cls(np.concatenate([[0], np.cumsum(np.asarray(lengths, dtype=np.int64))]).astype(np.int64), index)
+
+    @classmethod
+    def of_padded(cls, lengths, index, pitch):
+        """A padded batch ``[len(lengths) * pitch, channels]``: sentence ``s`` in the first ``lengths[s]`` of its rows."""
+        lengths, index = np.asarray(lengths, dtype=np.int64), np.asarray(index, dtype=np.int64)
+        if lengths.shape != index.shape or lengths.ndim != 1 or (lengths < 0).any() or (lengths > pitch).any():
+            raise ValueError(f"Segments: a length in [0, {pitch}] and an index for each sentence")
+        start = np.arange(lengths.size, dtype=np.int64) * pitch
+        off = np.stack([start, start + lengths], 1).reshape(-1)
+        return cls(np.append(off, lengths.size * pitch), np.stack([index, np.full_like(index, cls.SKIP)], 1).reshape(-1))
+
+    def covers(self, tokens):
+        """Whether every one of ``tokens`` tokens is somebody's."""
+        return self.whole and self.lo == 0 and self.hi == tokens
 
 
 class Operators:
@@ -218,7 +240,7 @@ class Operators:
         of_y = (tokens, cout)
         layout, (ldx, ldbase, ldy) = self._layout(False, (("x", x, (tokens, cin)), ("base", base, of_y), ("out", out, of_y)))
         seg = self._segments(seg, tokens)
-        full = seg.lo == 0 and seg.hi == tokens
+        full = seg.covers(tokens)
         if out is None:
             out, ldy = self._out(x, tokens, cout, layout, full)
         h = (torch.empty if full else torch.zeros)((tokens, rank), dtype=f32, device=x.device) if keep else None
@@ -245,7 +267,7 @@ class Operators:
         self._need("h", h, (tokens, rank))
         seg = self._segments(seg, tokens)
         if dx is None:
-            dx, lddx = self._out(x, tokens, cin, 0, seg.lo == 0 and seg.hi == tokens)
+            dx, lddx = self._out(x, tokens, cin, 0, seg.covers(tokens))
         da = torch.empty((n, rank, cin), dtype=f32, device=x.device)
         db = torch.empty((n, cout, rank), dtype=f32, device=x.device)
         p = _LORA_GRAD.pack(code, cin, cout, rank, n, tokens, x.data_ptr(), ldx, dy.data_ptr(), lddy, h.data_ptr(),
@@ -269,7 +291,7 @@ class Operators:
         self._need("gain", gain, (gains, c))
         self._need("offset", offset, (gains, c))
         seg = self._segments(seg, tokens)
-        full = seg.lo == 0 and seg.hi == tokens
+        full = seg.covers(tokens)
         if out is None:
             out, ldy = self._out(x, tokens, c, layout, full)
         mean = rstd = None
@@ -300,7 +322,7 @@ class Operators:
         self._need("rstd", rstd, (tokens,))
         seg = self._segments(seg, tokens)
         if dx is None:
-            dx, lddx = self._out(x, tokens, c, 0, seg.lo == 0 and seg.hi == tokens)
+            dx, lddx = self._out(x, tokens, c, 0, seg.covers(tokens))
         dgain = torch.empty((gains, c), dtype=f32, device=x.device)
         doffset = torch.empty((gains, c), dtype=f32, device=x.device)
         p = _NORM_GRAD.pack(code, c, gains, tokens, x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldres,
