@@ -263,6 +263,8 @@ int k82_op_lora(k82_handle* h, const k82_lora* p, const k82_segments* seg, void*
  *   dx = dx_base + scale[k] (dy B_k) A_k   (k = -1: dx = dx_base; dx_base NULL: 0; dx_base may be dx itself)
  *   da_k = scale[k] sum_t (dy B_k)^T x,  db_k = scale[k] sum_t dy^T h   (f32; zero for an adapter without tokens)
  * Sums over tokens are taken in a fixed order: the same call gives the same bits.  dx may not overlap x or dy.
+ * K82_BF16 takes h and dy B_k in parts, in the forward call too: an infinity of x, dy or a factor that meets them gives an
+ * infinity or a NaN, never a finite number.
  * workspace: device memory of at least k82_op_lora_grad_workspace bytes, 256-byte aligned, the caller's until the
  * enqueued work is done. */
 typedef struct k82_lora_grad {

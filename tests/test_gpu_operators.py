@@ -183,6 +183,34 @@ def test_lora_values_that_are_not_numbers_stay_in_their_token(ops, dt, kind):
     assert torch.equal(ops.op_lora(x, a_other, b, scale, only, base=base)[:5], clean[:5])
 
 
+@pytest.mark.parametrize("dt,kind", [(torch.float32, "dense"), (torch.float32, "cols"), (torch.bfloat16, "dense")])
+def test_infinities_come_through(ops, dt, kind):
+    """One rank, so no two infinities meet: the result is the definition's, sign by sign, and the gradient's too.
+
+    A factor's gradient in bf16 takes g and h in three parts.  An infinity of x or dy times parts of both signs is
+    inf - inf, so there, and there alone, a NaN may stand for the infinity; it is never a finite number."""
+    x, base, a, b, scale = lora_case(37, 64, 72, 1, 2, dt, kind, 91)
+    x[5, 9], x[20, 40] = float("inf"), -float("inf")
+    base[7, 3] = float("inf")
+    seg = Segments([0, 18, 37], [1, 0])
+    want = lora_want(x, base, a, b, scale, seg, "none")[0]
+    y, h = ops.op_lora(x, a, b, scale, seg, base=base, keep=True)
+    bad = ~torch.isfinite(want)
+    assert bad[5].all() and bad[20].all() and torch.equal(bad, ~torch.isfinite(y)) and torch.equal(y[bad].double(), want[bad])
+    if kind == "cols":
+        return
+    x, dy, a, b, scale = lora_case(37, 64, 72, 1, 2, dt, kind, 92)
+    _, h = ops.op_lora(x, a, b, scale, seg, keep=True)
+    dy[5, 9], h[30] = float("inf"), -float("inf")
+    got = ops.op_lora_grad(x, dy, h, a, b, scale, seg)
+    for name, g, (w, _) in zip(("dx", "da", "db"), got, lora_grad_want(x, dy, h, None, a, b, scale, seg)):
+        bad = ~torch.isfinite(w)
+        assert bad.any() and torch.equal(bad, ~torch.isfinite(g))
+        if dt == torch.bfloat16 and name == "db":
+            bad[1, 9] = False
+        assert torch.equal(g[bad].double().nan_to_num(nan=7.0), w[bad].nan_to_num(nan=7.0))
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_lora_into_the_shared_projections_own_buffer(ops, dt):
     x, base, a, b, scale = lora_case(90, 72, 136, 12, 3, dt, "dense", 4)
