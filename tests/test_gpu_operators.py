@@ -493,6 +493,21 @@ def test_layernorm_backward_leaves_and_zeroes_what_it_should(ops, dt):
     assert (dg == 0).all() and (db == 0).all()
 
 
+@pytest.mark.parametrize("c,dt", [(300, torch.float32), (768, torch.bfloat16), (1100, torch.bfloat16), (5000, torch.float32)])
+def test_layernorm_backward_of_a_large_constant_row(ops, c, dt):
+    """Every sum of it is exact, so its variance is 0; mean * rstd = 2^110 * 1e6 is an infinity that no channel has."""
+    x, _, gain, offset = norm_case(9, c, 2, dt, "dense", 61)
+    dy = tensor(gen(62), 9, c, dt)
+    x[4] = 2.0 ** 110
+    seg = Segments([0, 6, 9], [1, 0])
+    _, mean, rstd = ops.op_layernorm(x, gain, offset, seg, stats=True)
+    assert mean[4] == 2.0 ** 110 and abs(float(rstd[4]) - 1e6) <= 1e6 * 4 * U
+    got = ops.op_layernorm_grad(x, dy, gain, mean, rstd, seg)
+    for what, g, (w, bound) in zip(("dx", "dgain", "doffset"), got, norm_grad_want(x, None, dy, gain, mean, rstd, seg)):
+        assert torch.isfinite(g).all()
+        within(g, w, bound, what)
+
+
 def test_layernorm_gradients_against_differences(ops):
     """Central differences of the definition in 64 bits: step 1e-5, so 1e-10 of truncation and 1e-11 of rounding."""
     x, res, gain, offset = norm_case(40, 96, 2, torch.float32, "dense", 33)

@@ -301,8 +301,14 @@ __global__ __launch_bounds__(kThreads<W>) void norm_grad_kernel(RunTable rt, k82
             Vec<T>::unpack(rr[i], res);
             Vec<T>::unpack(rd[i], w[i]);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {                        // (channels behind the row: dy = 0 adds nothing)
-                xh[i][j] = (xh[i][j] + res[j] - m) * r;
+            for (int j = 0; j < N; ++j) xh[i][j] = (xh[i][j] + res[j] - m) * r;
+            if (left[i] < N) {                                   // channels behind the row add nothing, not 0 times an infinity
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (j >= left[i]) xh[i][j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
                 ag[i][j] = fmaf(w[i][j], xh[i][j], ag[i][j]);
                 ab[i][j] += w[i][j];
                 w[i][j] *= g[i][j];
