@@ -333,3 +333,5 @@ def test_the_scheduler_hands_adapters_to_their_sentences():
     seen.clear()
     s.synthesize(ids, [np.zeros(256, np.float32)] * 4)
     assert {v for w in seen.values() for v in w} == {"none given"}
+    with pytest.raises(ValueError, match="adapters names 3 sentences, there are 4"):
+        s.synthesize(ids, [np.zeros(256, np.float32)] * 4, adapters=names[:3])

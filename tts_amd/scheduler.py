@@ -169,6 +169,8 @@ class BatchSynthesizer:
         indices = list(range(n)) if indices is None else list(indices)
         speeds = [1.0] * n if speeds is None else list(speeds)
         seeds = list(range(n)) if seeds is None else list(seeds)
+        if adapters is not None and len(adapters) != n:
+            raise ValueError(f"adapters names {len(adapters)} sentences, there are {n}")
         counts = [len(x) + 2 for x in id_lists]
         out = {}
         batches = make_batches(indices, counts, self.max_batch, self.max_tokens)
