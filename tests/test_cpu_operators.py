@@ -217,6 +217,34 @@ def test_python_face_refuses_before_the_library():
         ops.op_lora_grad(x, torch.zeros(4, 6), torch.zeros(4, 2), a, b, s, Segments([0, 4], [1]))
 
 
+@pytest.mark.parametrize("call,wrong", [("op_lora", "x a b scale"), ("op_lora_grad", "x dy h a b scale"),
+                                        ("op_layernorm", "x gain offset"), ("op_layernorm_grad", "x dy gain mean rstd")])
+def test_python_face_names_what_is_missing(call, wrong):
+    ops = object.__new__(Operators)
+    ops.device, ops.h, ops.lib = -1, C.c_void_p(), _lib.load()
+    given = dict(x=torch.zeros(4, 8), a=torch.zeros(1, 2, 8), b=torch.zeros(1, 6, 2), scale=torch.ones(1), h=torch.zeros(4, 2),
+                 dy=torch.zeros(4, 6 if "lora" in call else 8), gain=torch.ones(1, 8), offset=torch.ones(1, 8),
+                 mean=torch.ones(4), rstd=torch.ones(4))
+    names = wrong.split()
+    for name in names:
+        with pytest.raises(TypeError, match=f"^{name} must be a torch tensor"):
+            getattr(ops, call)(**{**{n: given[n] for n in names}, name: None})
+        with pytest.raises(ValueError):
+            getattr(ops, call)(**{**{n: given[n] for n in names}, name: torch.tensor(1.0)})
+
+
+def test_python_face_refuses_numbers_that_do_not_fit():
+    ops = object.__new__(Operators)
+    ops.device, ops.h, ops.lib = -1, C.c_void_p(), _lib.load()
+    x, gain = torch.zeros(4, 8), torch.ones(1, 8)
+    for eps in (None, "1e-5"):
+        with pytest.raises(ValueError, match="does not fit"):
+            ops.op_layernorm(x, gain, gain, eps=eps)
+    wide = torch.empty(0, 1 << 31)                               # no memory behind it
+    with pytest.raises(ValueError, match="does not fit"):
+        ops.op_layernorm(wide, wide, wide, Segments([0], []))
+
+
 def test_packed_arguments_are_the_structs():
     from tts_amd import operators as O
     for packed, c in ((O._LORA, _lib.K82Lora), (O._LORA_GRAD, _lib.K82LoraGrad), (O._NORM, _lib.K82Layernorm), (O._NORM_GRAD, _lib.K82LayernormGrad)):

@@ -138,20 +138,21 @@ class Operators:
         # torch's default stream is handle 0, which the library takes for "the handle's own": name it hipStreamLegacy (1)
         return self._raw_stream(self.device) or 1
 
-    def _placed(self, dtype, named):
-        """Every tensor is one of this GPU and of ``dtype``."""
+    def _placed(self, dtype, named, optional=()):
+        """Every tensor is one of this GPU and of ``dtype``; those of ``optional`` may be None."""
         dev = self.device
-        for name, t in named:
-            if t is None:
-                continue
-            try:
-                at, dt = t.get_device(), t.dtype
-            except AttributeError:
-                raise TypeError(f"{name} must be a torch tensor on the GPU") from None
-            if at != dev:
-                raise ValueError(f"{name} must be on cuda:{dev}, it is on {t.device}")
-            if dt is not dtype:
-                raise TypeError(f"{name} is {dt}, {dtype} is needed")
+        for some, needed in ((named, True), (optional, False)):
+            for name, t in some:
+                if t is None and not needed:
+                    continue
+                try:
+                    at, dt = t.get_device(), t.dtype
+                except AttributeError:
+                    raise TypeError(f"{name} must be a torch tensor on the GPU") from None
+                if at != dev:
+                    raise ValueError(f"{name} must be on cuda:{dev}, it is on {t.device}")
+                if dt is not dtype:
+                    raise TypeError(f"{name} is {dt}, {dtype} is needed")
 
     def _code(self, x):
         code = self._codes.get(getattr(x, "dtype", None))
@@ -186,6 +187,13 @@ class Operators:
             return 1, [0 if v is None else v[3] if v[1] > 1 else max(1, v[0]) for v in found]
         raise ValueError("tensors must share one layout: unit stride along the channels" + (
             "" if rows_only else " (or along the tokens: channel-first)") + " and rows that do not overlap")
+
+    @staticmethod
+    def _packed(form, *values):
+        try:
+            return form.pack(*values)
+        except struct.error as e:
+            raise ValueError(f"an argument does not fit the library's: {e}") from None
 
     @staticmethod
     def _need(name, t, shape):
@@ -231,12 +239,12 @@ class Operators:
         ``h = x @ a[k].T`` in float32, which ``op_lora_grad`` takes."""
         torch = self._torch or self._bind()
         code, dt, f32 = self._code(x), x.dtype, torch.float32
-        self._placed(dt, (("x", x), ("a", a), ("b", b), ("base", base), ("out", out)))
+        self._placed(dt, (("x", x), ("a", a), ("b", b)), (("base", base), ("out", out)))
         self._placed(f32, (("scale", scale),))
         if act not in ACTS:
             raise ValueError(f"act must be one of {sorted(ACTS)}, not {act!r}")
         n, rank, cin, cout = self._factors(a, b, scale)
-        tokens = x.shape[0]
+        tokens = x.shape[0] if x.dim() else 0
         of_y = (tokens, cout)
         layout, (ldx, ldbase, ldy) = self._layout(False, (("x", x, (tokens, cin)), ("base", base, of_y), ("out", out, of_y)))
         seg = self._segments(seg, tokens)
@@ -244,8 +252,8 @@ class Operators:
         if out is None:
             out, ldy = self._out(x, tokens, cout, layout, full)
         h = (torch.empty if full else torch.zeros)((tokens, rank), dtype=f32, device=x.device) if keep else None
-        p = _LORA.pack(code, layout, ACTS[act], cin, cout, rank, n, tokens, x.data_ptr(), ldx, 0 if base is None else base.data_ptr(),
-                       ldbase, out.data_ptr(), ldy, a.data_ptr(), b.data_ptr(), scale.data_ptr(), 0 if h is None else h.data_ptr())
+        p = self._packed(_LORA, code, layout, ACTS[act], cin, cout, rank, n, tokens, x.data_ptr(), ldx, 0 if base is None else base.data_ptr(),
+                         ldbase, out.data_ptr(), ldy, a.data_ptr(), b.data_ptr(), scale.data_ptr(), 0 if h is None else h.data_ptr())
         rc = self._fn["lora"](self.h, p, seg.address, self._stream())
         if rc:
             self._check(rc)
@@ -257,10 +265,10 @@ class Operators:
         ``db`` are float32 sums over the tokens in a fixed order, zero for an adapter without tokens."""
         torch = self._torch or self._bind()
         code, dt, f32 = self._code(x), x.dtype, torch.float32
-        self._placed(dt, (("x", x), ("dy", dy), ("a", a), ("b", b), ("dx_base", dx_base), ("dx", dx)))
+        self._placed(dt, (("x", x), ("dy", dy), ("a", a), ("b", b)), (("dx_base", dx_base), ("dx", dx)))
         self._placed(f32, (("h", h), ("scale", scale)))
         n, rank, cin, cout = self._factors(a, b, scale)
-        tokens = x.shape[0]
+        tokens = x.shape[0] if x.dim() else 0
         of_x = (tokens, cin)
         _, (ldx, lddy, ldbase, lddx) = self._layout(True, (("x", x, of_x), ("dy", dy, (tokens, cout)), ("dx_base", dx_base, of_x),
                                                            ("dx", dx, of_x)))
@@ -270,9 +278,9 @@ class Operators:
             dx, lddx = self._out(x, tokens, cin, 0, seg.covers(tokens))
         da = torch.empty((n, rank, cin), dtype=f32, device=x.device)
         db = torch.empty((n, cout, rank), dtype=f32, device=x.device)
-        p = _LORA_GRAD.pack(code, cin, cout, rank, n, tokens, x.data_ptr(), ldx, dy.data_ptr(), lddy, h.data_ptr(),
-                            0 if dx_base is None else dx_base.data_ptr(), ldbase, dx.data_ptr(), lddx, a.data_ptr(),
-                            b.data_ptr(), scale.data_ptr(), da.data_ptr(), db.data_ptr())
+        p = self._packed(_LORA_GRAD, code, cin, cout, rank, n, tokens, x.data_ptr(), ldx, dy.data_ptr(), lddy, h.data_ptr(),
+                         0 if dx_base is None else dx_base.data_ptr(), ldbase, dx.data_ptr(), lddx, a.data_ptr(),
+                         b.data_ptr(), scale.data_ptr(), da.data_ptr(), db.data_ptr())
         self._with_workspace("lora_grad", p, seg, x)
         return dx, da, db
 
@@ -283,11 +291,11 @@ class Operators:
         ``stats``: returns ``(y, mean, rstd)`` (float32), which ``op_layernorm_grad`` takes."""
         torch = self._torch or self._bind()
         code = self._code(x)
-        self._placed(x.dtype, (("x", x), ("gain", gain), ("offset", offset), ("res", res), ("out", out)))
+        self._placed(x.dtype, (("x", x), ("gain", gain), ("offset", offset)), (("res", res), ("out", out)))
         shape = x.shape
         layout, (ldx, ldres, ldy) = self._layout(False, (("x", x, None), ("res", res, shape), ("out", out, shape)))
         tokens, c = shape
-        gains = gain.shape[0]
+        gains = gain.shape[0] if gain.dim() else 0
         self._need("gain", gain, (gains, c))
         self._need("offset", offset, (gains, c))
         seg = self._segments(seg, tokens)
@@ -298,9 +306,9 @@ class Operators:
         if stats:
             new = torch.empty if full else torch.zeros
             mean, rstd = (new((tokens,), dtype=torch.float32, device=x.device) for _ in range(2))
-        p = _NORM.pack(code, layout, c, gains, eps, tokens, x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldres,
-                       out.data_ptr(), ldy, gain.data_ptr(), offset.data_ptr(), 0 if mean is None else mean.data_ptr(),
-                       0 if rstd is None else rstd.data_ptr())
+        p = self._packed(_NORM, code, layout, c, gains, eps, tokens, x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldres,
+                         out.data_ptr(), ldy, gain.data_ptr(), offset.data_ptr(), 0 if mean is None else mean.data_ptr(),
+                         0 if rstd is None else rstd.data_ptr())
         rc = self._fn["layernorm"](self.h, p, seg.address, self._stream())
         if rc:
             self._check(rc)
@@ -311,12 +319,12 @@ class Operators:
         ``dy``, ``x`` or ``res`` itself; ``dgain`` and ``doffset`` are float32 sums over the tokens in a fixed order."""
         torch = self._torch or self._bind()
         code, f32 = self._code(x), torch.float32
-        self._placed(x.dtype, (("x", x), ("dy", dy), ("gain", gain), ("res", res), ("dx", dx)))
+        self._placed(x.dtype, (("x", x), ("dy", dy), ("gain", gain)), (("res", res), ("dx", dx)))
         self._placed(f32, (("mean", mean), ("rstd", rstd)))
         shape = x.shape
         _, (ldx, ldres, lddy, lddx) = self._layout(True, (("x", x, None), ("res", res, shape), ("dy", dy, shape), ("dx", dx, shape)))
         tokens, c = shape
-        gains = gain.shape[0]
+        gains = gain.shape[0] if gain.dim() else 0
         self._need("gain", gain, (gains, c))
         self._need("mean", mean, (tokens,))
         self._need("rstd", rstd, (tokens,))
@@ -325,9 +333,9 @@ class Operators:
             dx, lddx = self._out(x, tokens, c, 0, seg.covers(tokens))
         dgain = torch.empty((gains, c), dtype=f32, device=x.device)
         doffset = torch.empty((gains, c), dtype=f32, device=x.device)
-        p = _NORM_GRAD.pack(code, c, gains, tokens, x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldres,
-                            dy.data_ptr(), lddy, dx.data_ptr(), lddx, gain.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-                            dgain.data_ptr(), doffset.data_ptr())
+        p = self._packed(_NORM_GRAD, code, c, gains, tokens, x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldres,
+                         dy.data_ptr(), lddy, dx.data_ptr(), lddx, gain.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                         dgain.data_ptr(), doffset.data_ptr())
         self._with_workspace("layernorm_grad", p, seg, x)
         return dx, dgain, doffset
 
