@@ -225,7 +225,9 @@ int k82_pcm16_static(k82_handle* h, const float* src, int16_t* dst, int64_t n, v
  * Segments cut the token axis: segment s holds the tokens [off[s], off[s+1]), 0 <= off[0] <= ... <= off[n] <= tokens,
  * and uses adapter (gain) index[s]; an index may come any number of times and a segment may be empty.  K82_SKIP (the padding
  * of a padded batch): its tokens belong to nobody.  Output rows that no segment holds, or a skipped one, are left as they
- * were, and what lies in the inputs there reaches no result. */
+ * were, and what lies in the inputs there reaches no result.
+ * An output shares no memory with another tensor of the call but where the call names one it may be; of tensors with a row for
+ * each token that is checked. */
 #define K82_SKIP (-2)
 #define K82_F32 0
 #define K82_BF16 1

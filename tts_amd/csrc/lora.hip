@@ -458,19 +458,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
             f4 d[TT];
 #pragma unroll
             for (int t = 0; t < TT; ++t) d[t] = f4{base[0][t], base[1][t], base[2][t], base[3][t]};
-            raw4 tb[RT];
+            raw4 fb[RT];
             if (k >= 0) {
 #pragma unroll
                 for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fac[r]);
                 wave_fence();
 #pragma unroll
-                for (int r = 0; r < RT; ++r) tb[r] = get_tile(own + r * 64);
+                for (int r = 0; r < RT; ++r) fb[r] = get_tile(own + r * 64);
                 wave_fence();
             }
             if (blk + stride < blocks) fetch(blk + stride);      // the next block is on its way while this one is multiplied
             if (k >= 0)
 #pragma unroll
-                for (int t = 0; t < TT; ++t) d[t] = h[t].times(tb, d[t]);
+                for (int t = 0; t < TT; ++t) d[t] = h[t].times(fb, d[t]);
             char* yb = (char*)p.y + (int64_t)16 * blk * p.ldy * 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
