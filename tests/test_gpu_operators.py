@@ -237,6 +237,19 @@ def test_lora_of_a_token_does_not_depend_on_its_batch(ops):
         assert torch.equal(whole[57:190], alone)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rank,cin,cout", [(33, 72, 40), (64, 64, 136), (128, 200, 24), (100, 37, 51)])
+def test_lora_of_many_tokens_takes_larger_tiles(ops, dt, rank, cin, cout):
+    """From 32768 tokens on: the definition, and the bits of the same tokens in a small call."""
+    tokens, seg = 33001, Segments([0, 5, 100, 20063, 33001], [2, 0, -1, 1])
+    check_lora(ops, tokens, cin, cout, rank, 3, dt, "dense", seg, seed=rank)
+    x, base, a, b, scale = lora_case(tokens, cin, cout, rank, 3, dt, "dense", 17)
+    y, h = ops.op_lora(x, a, b, scale, seg, base=base, keep=True)
+    for lo, hi, k in ((5, 100, 0), (20063, 20200, 1), (32950, 33001, 1)):
+        alone = ops.op_lora(x[lo:hi], a, b, scale, Segments([0, hi - lo], [k]), base=base[lo:hi], keep=True)
+        assert torch.equal(alone[0], y[lo:hi]) and torch.equal(alone[1], h[lo:hi])
+
+
 def lora_grad_want(x, dy, h, dx_base, a, b, scale, seg):
     dt = x.dtype
     (tokens, cin), cout, rank = x.shape, dy.shape[1], a.shape[1]

@@ -121,6 +121,16 @@ template <class T, int RT> __device__ __forceinline__ raw4 get_factor(const raw4
     } else return get_tile(tile);
 }
 
+// two tiles side by side, 128 bytes of each row: the 16 bytes of the row 8 e + lane / 8; tile e as the operand
+__device__ __forceinline__ void put_pair(raw4* tiles, int e, raw4 v) {
+    const int lane = threadIdx.x & 63;
+    tiles[64 * e + (lane & ~7) + ((lane & 7) ^ (lane >> 3))] = v;
+}
+__device__ __forceinline__ raw4 get_pair(const raw4* tiles, int e) {
+    const int col = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    return tiles[8 * col + ((4 * e + g) ^ (col & 7))];
+}
+
 // The sum over the waves' parts of k, and what follows from it for every wave: h for the second product, and h itself if kept.
 // tok: the token of this lane's column.
 template <class T, int NW, int RT, int TT>
@@ -162,17 +172,19 @@ constexpr int most(int a, int b) { return a > b ? a : b; }
 constexpr int kPad = 4;                        // floats behind a row of the results' tile: rows start on different banks
 
 // Token rows.  A workgroup takes 16 TT tokens of a segment; its NW waves share the k of the first product (each takes every
-// NW-th 64 bytes of a row, so together they read 64 NW contiguous bytes) and the output channels of the second, 128 bytes of a
+// NW-th 128 bytes of a row: whole lines; 64 bytes were 139 us where these are 133 below, and 16 cache lines a load, not 8) and the output channels of the second, 128 bytes of a
 // row a wave at a time.  The results cross LDS once more, so that base and y are read and written in whole lines.
 // blockIdx.y splits the output channels where there are few tokens; each part then computes h for itself, from cache.
 // EVEN: cin, cout and rank are multiples of a lane's 16 bytes, no place lies in part behind a row.
-// (waves_per_eu: without it the accumulators of four and eight rank tiles are copied through the second register file and one
-// wave less fits a SIMD; 65536 tokens 2048 -> 768 bf16 rank 64: 146 us, with it 137.)
+// A step's registers are loaded again as soon as LDS has its operands; a second step in flight fits only one rank tile (with
+// two it spilled: 65536 tokens 768 -> 768 bf16 rank 32 81 us, without 64).
+// 65536 tokens 2048 -> 768 bf16 rank 64 with TT = 4: 127 us of 473 MB, 3.7 TB/s (a large copy: 4.7).
+// (waves_per_eu: without it accumulators are copied through the second register file and a wave less fits a SIMD.)
 template <class T, int NW, int RT, int TT, bool EVEN>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8 ? 1 : RT >= 4 ? 3 : 4))) void lora_rows_kernel(SegTable sg, k82_lora p) {
-    constexpr int V = Vec<T>::N, K = 4 * V, S = sizeof(T), U = RT + TT > 4 ? 2 : 4;          // U: steps whose loads are in flight together
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8 ? 1 : RT >= 4 ? 2 : 4))) void lora_rows_kernel(SegTable sg, k82_lora p) {
+    constexpr int V = Vec<T>::N, K = 4 * V, K2 = 2 * K, S = sizeof(T), U = RT > 1 ? 1 : 2;          // a step: 128 bytes of a row; U of them in flight
     constexpr int CH = 8 * V, MT = CH / 16, CK = Second<T, RT>::CHUNKS;          // channels, row tiles of B, chunks of a row of B
-    constexpr int kTiles = most(RT + TT, MT * CK), kRow = CH + kPad;
+    constexpr int kTiles = most(2 * (RT + TT), MT * CK), kRow = CH + kPad;
     constexpr int kOwn = most(kTiles * 1024, MT * CK * 1024 + 16 * kRow * 4);    // a wave's own bytes
     __shared__ __align__(16) char lds[most(NW * kOwn, NW * RT * TT * 1024)];
     const int s = seg_of(sg, blockIdx.x), k = sg.index[s];
@@ -213,59 +225,81 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
     if (k >= 0) {
         f4 acc[RT][TT];
         const char *ap = (const char*)p.a + (int64_t)k * p.rank * p.cin * S, *xp = (const char*)p.x + t0 * p.ldx * S;
-        uint32_t ao[RT], xo[TT];
+        uint32_t ao[RT][2], xo[TT][2];                           // this lane's 16 bytes of the rows (lane / 8) and + 8 of a tile
 #pragma unroll
-        for (int r = 0; r < RT; ++r) ao[r] = (min(rank_of<T, RT>(r, lane >> 2), p.rank - 1) * (uint32_t)p.cin + c4) * S;
+        for (int e = 0; e < 2; ++e) {
+            const int row = 8 * e + (lane >> 3);
 #pragma unroll
-        for (int t = 0; t < TT; ++t) xo[t] = (min(16 * t + (lane >> 2), last) * (uint32_t)p.ldx + c4) * S;
+            for (int r = 0; r < RT; ++r) ao[r][e] = (min(rank_of<T, RT>(r, row), p.rank - 1) * (uint32_t)p.cin + c8) * S;
+#pragma unroll
+            for (int t = 0; t < TT; ++t) xo[t][e] = (min(16 * t + row, last) * (uint32_t)p.ldx + c8) * S;
+        }
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int t = 0; t < TT; ++t) acc[r][t] = f4{0.f, 0.f, 0.f, 0.f};
-        auto multiply = [&](const raw4 (&fa)[RT], const raw4 (&fx)[TT]) {
+        raw4 fa[U][RT][2], fx[U][TT][2];
+        const int full = p.cin / K2;
+        auto load = [&](int u, int i) {
+            const int at = i * K2 * S;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fa[r]);
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int t = 0; t < TT; ++t) put_tile(own + (RT + t) * 64, fx[t]);
-            wave_fence();
-            raw4 ta[RT], tx[TT];
+                for (int t = 0; t < TT; ++t) fx[u][t][e] = load16(xp + at, xo[t][e]);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) ta[r] = get_tile(own + r * 64);
-#pragma unroll
-            for (int t = 0; t < TT; ++t) tx[t] = get_tile(own + (RT + t) * 64);
-            wave_fence();
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int t = 0; t < TT; ++t) acc[r][t] = product<T>(ta[r], tx[t], acc[r][t]);
-        };
-        const int full = p.cin / K;
-        auto steps = [&](int i0, auto n) {
-            constexpr int n_ = decltype(n)::value;
-            raw4 fa[n_][RT], fx[n_][TT];
-#pragma unroll
-            for (int i = 0; i < n_; ++i) {
-                const int at = (i0 + i * NW) * K * S;
-#pragma unroll
-                for (int t = 0; t < TT; ++t) fx[i][t] = load16(xp + at, xo[t]);
-#pragma unroll
-                for (int r = 0; r < RT; ++r) fa[i][r] = load16(ap + at, ao[r]);
+                for (int r = 0; r < RT; ++r) fa[u][r][e] = load16(ap + at, ao[r][e]);
             }
+            __builtin_amdgcn_sched_barrier(0);                   // (the compiler would gather the loads of several steps)
+        };
+        // step u of the ring, whose place then takes step `next` (sure: there is one)
+        auto multiply = [&](int u, int next, auto sure) {
 #pragma unroll
-            for (int i = 0; i < n_; ++i) multiply(fa[i], fx[i]);
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int t = 0; t < TT; ++t) put_pair(own + t * 128, e, fx[u][t][e]);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) put_pair(own + (TT + r) * 128, e, fa[u][r][e]);
+            }
+            if (decltype(sure)::value || next < full) load(u, next);
+            wave_fence();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                raw4 ta[RT], tx[TT];
+#pragma unroll
+                for (int t = 0; t < TT; ++t) tx[t] = get_pair(own + t * 128, e);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) ta[r] = get_pair(own + (TT + r) * 128, e);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) acc[r][t] = product<T>(ta[r], tx[t], acc[r][t]);
+            }
+            wave_fence();
         };
         int i = wave;
-        for (; i + (U - 1) * NW < full; i += U * NW) steps(i, std::integral_constant<int, U>());
-        if (U > 2 && i + NW < full) { steps(i, std::integral_constant<int, 2>()); i += 2 * NW; }
-        if (i < full) { steps(i, std::integral_constant<int, 1>()); i += NW; }
-        if (i == full && p.cin % K) {                            // one wave: the end of the row, zeros behind it
-            const int at = full * K, n = p.cin - at - c4;
-            raw4 fa[RT], fx[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) fx[t] = grab<T, EVEN>(xp + at * S, xo[t], n, c4 * S);
+        for (int u = 0; u < U; ++u)
+            if (i + u * NW < full) load(u, i + u * NW);
+        for (; i + (2 * U - 1) * NW < full; i += U * NW) {
 #pragma unroll
-            for (int r = 0; r < RT; ++r) fa[r] = grab<T, EVEN>(ap + at * S, ao[r], n, c4 * S);
-            multiply(fa, fx);
+            for (int u = 0; u < U; ++u) multiply(u, i + (U + u) * NW, std::true_type());
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i < full) { multiply(u, i + U * NW, std::false_type()); i += NW; }
+#pragma unroll
+        for (int u = 0; u < U - 1; ++u)
+            if (i < full) { multiply(u, full, std::false_type()); i += NW; }
+        if (i == full && p.cin % K2) {                           // one wave: the end of the row, zeros behind it
+            const int at = full * K2 * S, n = p.cin - full * K2 - c8;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int t = 0; t < TT; ++t) fx[0][t][e] = grab<T, EVEN>(xp + at, xo[t][e], n, c8 * S);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) fa[0][r][e] = grab<T, EVEN>(ap + at, ao[r][e], n, c8 * S);
+            }
+            multiply(0, full, std::false_type());
         }
         int64_t tok[TT];
         bool in[TT];
@@ -723,6 +757,10 @@ template <class F> hipError_t by_rank(int rank, F&& f) {
 // parts cost more first products than their balance gains: 16411 x 768 f32 channel-first 48 us, with up to 1100 workgroups 56.
 int parts(int tiles, int cout, int wide) { return std::max(1, std::min((cout + wide - 1) / wide, 512 / std::max(1, tiles))); }
 
+// 64 tokens a workgroup instead of 32, once that leaves two workgroups a CU: the factors are read half as often, which counts
+// where there are more ranks than tokens of a tile.  65536 tokens 768 -> 768 bf16 rank 64 71 us (32 tokens: 84), rank 128 143
+// (174), f32 rank 64 170 (187); with one rank tile 16411 tokens 768 -> 2048 52 (45), 16384 tokens rank 64 32 (21).
+template <class T, int RT> constexpr bool kLargeTiles = RT >= 4;
 template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::Seg>& segs, hipStream_t st) {
     return by_rank(p.rank, [&](auto rt) -> hipError_t {
         constexpr int RT = decltype(rt)::value, V = Vec<T>::N;
@@ -742,13 +780,21 @@ template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::S
                 // pairs of tokens a lane (128 bytes of a channel a tile), where there is a pair
                 return p.tokens >= 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
             }
-        constexpr int TT = 2, NW = 4;
-        for (const SegTable& t : op::tables(segs, 16 * TT)) {
-            const int tiles = t.tile0[t.n];
-            OP_TRY(op::run(even ? lora_rows_kernel<T, NW, RT, TT, true> : lora_rows_kernel<T, NW, RT, TT, false>,
-                           dim3(tiles, parts(tiles, p.cout, 8 * NW * V)), dim3(64 * NW), 0, st, t, p));
+        auto go = [&](auto tt) -> hipError_t {
+            constexpr int TT = decltype(tt)::value, NW = 4;
+            for (const SegTable& t : op::tables(segs, 16 * TT)) {
+                const int tiles = t.tile0[t.n];
+                OP_TRY(op::run(even ? lora_rows_kernel<T, NW, RT, TT, true> : lora_rows_kernel<T, NW, RT, TT, false>,
+                               dim3(tiles, parts(tiles, p.cout, 8 * NW * V)), dim3(64 * NW), 0, st, t, p));
+            }
+            return hipSuccess;
+        };
+        if constexpr (kLargeTiles<T, RT>) {
+            int64_t tokens = 0;
+            for (const op::Seg& g : segs) tokens += g.len;
+            if (tokens >= 64 * 512) return go(std::integral_constant<int, 4>());
         }
-        return hipSuccess;
+        return go(std::integral_constant<int, 2>());
     });
 }
 
