@@ -166,17 +166,23 @@ class Operators:
     def _layout(rows_only, shapes):
         """-> (layout, [ld of each]) of [tokens, channels] tensors that share one layout; shapes: (name, tensor or None,
         wanted shape or None)."""
-        rows, cols, found = True, not rows_only, []
+        rows, cols, found, plain = True, not rows_only, [], True
         for name, t, want in shapes:
             if t is None:
-                found.append(None)
                 continue
             shape = t.shape
             if len(shape) != 2:
                 raise ValueError(f"{name} must have two dimensions [tokens, channels], it has {len(shape)}")
             if want is not None and shape != want:
                 raise ValueError(f"{name} has shape {tuple(shape)}, {tuple(want)} is needed")
-            n, c = shape
+            plain = plain and t.is_contiguous()
+        if plain:                                                # the common case in half the time
+            return 0, [0 if t is None else t.shape[1] or 1 for _, t, _ in shapes]
+        for name, t, want in shapes:
+            if t is None:
+                found.append(None)
+                continue
+            n, c = t.shape
             sn, sc = t.stride()
             rows = rows and (sc == 1 or c == 1) and (n <= 1 or sn >= c)
             cols = cols and (sn == 1 or n == 1) and (c <= 1 or sc >= n)
@@ -197,18 +203,16 @@ class Operators:
 
     @staticmethod
     def _need(name, t, shape):
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{name} has shape {tuple(t.shape)}, {shape} is needed")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
 
     def _out(self, x, n, channels, cols, full):
         """A new [tokens, channels] tensor in the layout of x and its ld; zero where no segment will write."""
-        new = self._torch.empty if full else self._torch.zeros
-        if cols:
-            ld = max(32, (n + 31) // 32 * 32)
-            return new((channels, ld), dtype=x.dtype, device=x.device).t()[:n], ld
-        return new((n, channels), dtype=x.dtype, device=x.device), channels
+        ld = max(32, (n + 31) // 32 * 32) if cols else channels
+        out = x.new_empty_strided((n, channels), (1, ld)) if cols else x.new_empty((n, channels))
+        return out if full else out.zero_(), ld
 
     @staticmethod
     def _segments(seg, n):
@@ -221,10 +225,11 @@ class Operators:
         return seg
 
     def _factors(self, a, b, scale):
-        if a.dim() != 3 or b.dim() != 3:
+        of_a, of_b = a.shape, b.shape
+        if len(of_a) != 3 or len(of_b) != 3:
             raise ValueError("a is [adapters, rank, cin] and b [adapters, cout, rank]")
-        n, rank, cin = a.shape
-        cout = b.shape[1]
+        n, rank, cin = of_a
+        cout = of_b[1]
         self._need("b", b, (n, cout, rank))
         self._need("scale", scale, (n,))
         if not a.is_contiguous():
@@ -251,7 +256,9 @@ class Operators:
         full = seg.covers(tokens)
         if out is None:
             out, ldy = self._out(x, tokens, cout, layout, full)
-        h = (torch.empty if full else torch.zeros)((tokens, rank), dtype=f32, device=x.device) if keep else None
+        h = scale.new_empty((tokens, rank)) if keep else None
+        if keep and not full:
+            h.zero_()
         p = self._packed(_LORA, code, layout, ACTS[act], cin, cout, rank, n, tokens, x.data_ptr(), ldx, 0 if base is None else base.data_ptr(),
                          ldbase, out.data_ptr(), ldy, a.data_ptr(), b.data_ptr(), scale.data_ptr(), 0 if h is None else h.data_ptr())
         rc = self._fn["lora"](self.h, p, seg.address, self._stream())
@@ -276,8 +283,7 @@ class Operators:
         seg = self._segments(seg, tokens)
         if dx is None:
             dx, lddx = self._out(x, tokens, cin, 0, seg.covers(tokens))
-        da = torch.empty((n, rank, cin), dtype=f32, device=x.device)
-        db = torch.empty((n, cout, rank), dtype=f32, device=x.device)
+        da, db = scale.new_empty((n, rank, cin)), scale.new_empty((n, cout, rank))
         p = self._packed(_LORA_GRAD, code, cin, cout, rank, n, tokens, x.data_ptr(), ldx, dy.data_ptr(), lddy, h.data_ptr(),
                          0 if dx_base is None else dx_base.data_ptr(), ldbase, dx.data_ptr(), lddx, a.data_ptr(),
                          b.data_ptr(), scale.data_ptr(), da.data_ptr(), db.data_ptr())
@@ -331,8 +337,7 @@ class Operators:
         seg = self._segments(seg, tokens)
         if dx is None:
             dx, lddx = self._out(x, tokens, c, 0, seg.covers(tokens))
-        dgain = torch.empty((gains, c), dtype=f32, device=x.device)
-        doffset = torch.empty((gains, c), dtype=f32, device=x.device)
+        dgain, doffset = mean.new_empty((gains, c)), mean.new_empty((gains, c))
         p = self._packed(_NORM_GRAD, code, c, gains, tokens, x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldres,
                          dy.data_ptr(), lddy, dx.data_ptr(), lddx, gain.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                          dgain.data_ptr(), doffset.data_ptr())
