@@ -49,6 +49,20 @@ template <class T, bool EVEN> __device__ __forceinline__ raw4 grab(const char* b
         return n > 0 ? r : zero;
     } else return n > 0 ? load_part((const T*)(base + at), n) : raw4{0u, 0u, 0u, 0u};
 }
+// the elements 0, ld, 2 ld ... of p as 16 bytes: n of them at most, zeros behind
+template <class T> __device__ __forceinline__ raw4 across(const T* p, int ld, int n) {
+    constexpr int N = Vec<T>::N;
+    T v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = j < n ? p[j * (uint32_t)ld] : T(0);
+    raw4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (N == 4) r[j] = __float_as_uint(v[j]);
+        else r[j] = v[2 * j] | (uint32_t)v[2 * j + 1] << 16;
+    }
+    return r;
+}
 __device__ __forceinline__ void put_tile(raw4* tile, raw4 v) {
     const int lane = threadIdx.x & 63;
     tile[(lane & ~3) + ((lane & 3) ^ (lane >> 4))] = v;
@@ -180,7 +194,8 @@ constexpr int kPad = 4;                        // floats behind a row of the res
 // two it spilled: 65536 tokens 768 -> 768 bf16 rank 32 81 us, without 64).
 // 65536 tokens 2048 -> 768 bf16 rank 64 with TT = 4: 127 us of 473 MB, 3.7 TB/s (a large copy: 4.7).
 // (waves_per_eu: without it accumulators are copied through the second register file and a wave less fits a SIMD.)
-template <class T, int NW, int RT, int TT, bool EVEN>
+// ACROSS: a is [adapters][cin][rank] and b [adapters][rank][cout], read element by element (the backward pass of one rank tile).
+template <class T, int NW, int RT, int TT, bool EVEN, bool ACROSS = false>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8 ? 1 : RT >= 4 ? 2 : 4))) void lora_rows_kernel(SegTable sg, k82_lora p) {
     constexpr int V = Vec<T>::N, K = 4 * V, K2 = 2 * K, S = sizeof(T), U = RT > 1 ? 1 : 2;          // a step: 128 bytes of a row; U of them in flight
     constexpr int CH = 8 * V, MT = CH / 16, CK = Second<T, RT>::CHUNKS;          // channels, row tiles of B, chunks of a row of B
@@ -211,10 +226,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
         if (k >= 0) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const uint32_t at = (min(16 * m + (lane >> 2), n - 1) * (uint32_t)p.rank + c4) * S;
+                const int row = min(16 * m + (lane >> 2), n - 1);
+                const uint32_t at = (row * (uint32_t)p.rank + c4) * S;
 #pragma unroll
                 for (int c = 0; c < CK; ++c)
-                    fac[m * CK + c] = grab<T, EVEN>(bp + (int64_t)blk * CH * p.rank * S, at + c * K * S, p.rank - c * K - c4, (c * K + c4) * S);
+                    if constexpr (ACROSS) fac[m * CK + c] = across((const T*)(bp + (int64_t)blk * CH * S) + row + (uint32_t)(c * K + c4) * p.cout, p.cout, p.rank - c * K - c4);
+                    else fac[m * CK + c] = grab<T, EVEN>(bp + (int64_t)blk * CH * p.rank * S, at + c * K * S, p.rank - c * K - c4, (c * K + c4) * S);
             }
         }
     };
@@ -230,7 +247,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
         for (int e = 0; e < 2; ++e) {
             const int row = 8 * e + (lane >> 3);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) ao[r][e] = (min(rank_of<T, RT>(r, row), p.rank - 1) * (uint32_t)p.cin + c8) * S;
+            for (int r = 0; r < RT; ++r) {
+                const uint32_t k = min(rank_of<T, RT>(r, row), p.rank - 1);
+                ao[r][e] = (ACROSS ? c8 * (uint32_t)p.rank + k : k * (uint32_t)p.cin + c8) * S;
+            }
 #pragma unroll
             for (int t = 0; t < TT; ++t) xo[t][e] = (min(16 * t + row, last) * (uint32_t)p.ldx + c8) * S;
         }
@@ -247,7 +267,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
 #pragma unroll
                 for (int t = 0; t < TT; ++t) fx[u][t][e] = load16(xp + at, xo[t][e]);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) fa[u][r][e] = load16(ap + at, ao[r][e]);
+                for (int r = 0; r < RT; ++r) {
+                    if constexpr (ACROSS) fa[u][r][e] = across((const T*)(ap + (int64_t)at * p.rank + ao[r][e]), p.rank, V);
+                    else fa[u][r][e] = load16(ap + at, ao[r][e]);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);                   // (the compiler would gather the loads of several steps)
         };
@@ -297,7 +320,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
 #pragma unroll
                 for (int t = 0; t < TT; ++t) fx[0][t][e] = grab<T, EVEN>(xp + at, xo[t][e], n, c8 * S);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) fa[0][r][e] = grab<T, EVEN>(ap + at, ao[r][e], n, c8 * S);
+                for (int r = 0; r < RT; ++r) {
+                    if constexpr (ACROSS) fa[0][r][e] = across((const T*)(ap + (int64_t)at * p.rank + ao[r][e]), p.rank, n);
+                    else fa[0][r][e] = grab<T, EVEN>(ap + at, ao[r][e], n, c8 * S);
+                }
             }
             multiply(0, full, std::false_type());
         }
@@ -578,7 +604,7 @@ __device__ __forceinline__ void split3(const float (&v)[8], raw4& hi, raw4& mid,
 // More than 32 ranks are shares of neighbouring workgroups (their sums would leave one wave a SIMD): the channels come from the
 // shared cache again, 65536 tokens 768 / 2048 rank 64 130 us, with the shares one after the other 173.
 template <class T, int RT, bool EVEN>
-__global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k82_lora_grad p, const float* gs, const float* scales, int used0, float* part) {
+__global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k82_lora_grad p, const float* gs, float* part) {
     constexpr int V = Vec<T>::N, M = 8, S = sizeof(T);           // M: 16 x 16 tiles along the channels
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int chunk = rt.chunk0[0] + (int)blockIdx.y, run = place(rt.chunk0, chunk);
@@ -686,7 +712,7 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
         }
     }
     // row 4 g + i of tile m is the channel 8 (4 g + i) + m (bf16) or 64 (m / 4) + 4 (4 g + i) + m % 4 (f32)
-    const float scale = scales[used0 + run];
+    const float scale = p.scale[rt.index[run]];
     float* out = part + (int64_t)chunk * p.rank * (p.cin + p.cout) + (of_x ? 0 : p.cin);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -702,49 +728,47 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
             }
     }
 }
-// da, db: the chunks of an adapter in order.  64 channels x 16 ranks a workgroup; db's ranks leave side by side, through LDS.
-__global__ __launch_bounds__(256) void lora_reduce_kernel(ReduceTable rt, int cin, int cout, int rank, const float* part, float* da, float* db) {
-    __shared__ float tile[64][17];
+// da, db: the chunks of an adapter, 64 channels x 16 ranks a workgroup.  Four shares of four waves take every fourth chunk in
+// order, and their sums join in order (4096 tokens of one adapter, 768 / 768 bf16 rank 8, 85 chunks:
+// the backward pass 48 us with one share, 29 with four).
+// db's ranks leave side by side.
+__global__ __launch_bounds__(1024) void lora_reduce_kernel(ReduceTable rt, int cin, int cout, int rank, const float* part, float* da, float* db) {
+    __shared__ float tile[4][64][17];
     const int nx = (cin + 63) / 64, k = blockIdx.z, r0 = 16 * blockIdx.y;
     const bool of_x = (int)blockIdx.x < nx;
-    const int width = of_x ? cin : cout, c = 64 * ((int)blockIdx.x - (of_x ? 0 : nx)) + ((int)threadIdx.x & 63);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = wave & 3, share = wave >> 2;
+    const int width = of_x ? cin : cout, c0 = 64 * ((int)blockIdx.x - (of_x ? 0 : nx)), c = c0 + lane;
     const int64_t step = (int64_t)rank * (cin + cout);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < width) {
-        const float* q = part + (int64_t)rt.first[k] * step + (of_x ? 0 : cin) + c;
+        const float* q = part + (int64_t)(rt.first[k] + share) * step + (of_x ? 0 : cin) + c;
         int64_t row[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) row[j] = (int64_t)min(r0 + ((int)threadIdx.x >> 6) + 4 * j, rank - 1) * (cin + cout);
-        int n = rt.first[k + 1] - rt.first[k];
-        for (; n >= 2; n -= 2, q += 2 * step) {                  // (eight loads at once, added in order)
+        for (int j = 0; j < 4; ++j) row[j] = (int64_t)min(r0 + group + 4 * j, rank - 1) * (cin + cout);
+        int n = (rt.first[k + 1] - rt.first[k] - share + 3) / 4;
+        for (; n >= 2; n -= 2, q += 8 * step) {                  // (eight loads at once, added in order)
             float v[2][4];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[i][j] = q[i * step + row[j]];
+                for (int j = 0; j < 4; ++j) v[i][j] = q[4 * i * step + row[j]];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[j] += v[i][j];
         }
-        if (n)
+        if (n > 0)
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[j] += q[row[j]];
     }
-    if (of_x) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = r0 + ((int)threadIdx.x >> 6) + 4 * j;
-            if (c < width && r < rank) da[((int64_t)(rt.base + k) * rank + r) * cin + c] = s[j];
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) tile[threadIdx.x & 63][((int)threadIdx.x >> 6) + 4 * j] = s[j];
+    for (int j = 0; j < 4; ++j) tile[share][lane][group + 4 * j] = s[j];
     __syncthreads();
-    const int r = threadIdx.x & 15, o0 = 64 * ((int)blockIdx.x - nx);
-    for (int i = threadIdx.x >> 4; i < 64; i += 16)
-        if (o0 + i < cout && r0 + r < rank) db[((int64_t)(rt.base + k) * cout + o0 + i) * rank + r0 + r] = tile[i][r];
+    const int r = of_x ? wave : threadIdx.x & 15, i = of_x ? lane : threadIdx.x >> 4;
+    if (c0 + i >= width || r0 + r >= rank) return;
+    const float sum = ((tile[0][i][r] + tile[1][i][r]) + tile[2][i][r]) + tile[3][i][r];
+    if (of_x) da[((int64_t)(rt.base + k) * rank + r0 + r) * cin + c0 + i] = sum;
+    else db[((int64_t)(rt.base + k) * cout + c0 + i) * rank + r0 + r] = sum;
 }
 
 template <class F> hipError_t by_rank(int rank, F&& f) {
@@ -761,7 +785,7 @@ int parts(int tiles, int cout, int wide) { return std::max(1, std::min((cout + w
 // where there are more ranks than tokens of a tile.  65536 tokens 768 -> 768 bf16 rank 64 71 us (32 tokens: 84), rank 128 143
 // (174), f32 rank 64 170 (187); with one rank tile 16411 tokens 768 -> 2048 52 (45), 16384 tokens rank 64 32 (21).
 template <class T, int RT> constexpr bool kLargeTiles = RT >= 4;
-template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::Seg>& segs, hipStream_t st) {
+template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::Seg>& segs, hipStream_t st, bool across = false) {
     return by_rank(p.rank, [&](auto rt) -> hipError_t {
         constexpr int RT = decltype(rt)::value, V = Vec<T>::N;
         const bool even = p.cin % V == 0 && p.cout % V == 0 && p.rank % V == 0;
@@ -784,15 +808,17 @@ template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::S
             constexpr int TT = decltype(tt)::value, NW = 4;
             for (const SegTable& t : op::tables(segs, 16 * TT)) {
                 const int tiles = t.tile0[t.n];
-                OP_TRY(op::run(even ? lora_rows_kernel<T, NW, RT, TT, true> : lora_rows_kernel<T, NW, RT, TT, false>,
-                               dim3(tiles, parts(tiles, p.cout, 8 * NW * V)), dim3(64 * NW), 0, st, t, p));
+                auto kernel = even ? lora_rows_kernel<T, NW, RT, TT, true> : lora_rows_kernel<T, NW, RT, TT, false>;
+                if constexpr (RT == 1 && V == 4)
+                    if (across) kernel = even ? lora_rows_kernel<T, NW, RT, TT, true, true> : lora_rows_kernel<T, NW, RT, TT, false, true>;
+                OP_TRY(op::run(kernel, dim3(tiles, parts(tiles, p.cout, 8 * NW * V)), dim3(64 * NW), 0, st, t, p));
             }
             return hipSuccess;
         };
         if constexpr (kLargeTiles<T, RT>) {
             int64_t tokens = 0;
             for (const op::Seg& g : segs) tokens += g.len;
-            if (tokens >= 64 * 512) return go(std::integral_constant<int, 4>());
+            if (!across && tokens >= 64 * 512) return go(std::integral_constant<int, 4>());
         }
         return go(std::integral_constant<int, 2>());
     });
@@ -810,9 +836,13 @@ int chunk_rows(const k82_lora_grad& p, int64_t tokens) {
     const int64_t chunks = std::max<int64_t>(1, (p.rank <= 16 ? 512 : 768) / weight_groups(p));
     return (int)std::max<int64_t>(32, ((tokens + chunks - 1) / chunks + 31) / 32 * 32);
 }
+// One rank tile in f32: the factors are read across instead of being transposed first, a launch less (211 tokens 768 -> 768 rank
+// 7 20 us, transposed 21 to 23; 16384 tokens 73 and 76).  Not in bf16, eight loads for 16 bytes (16384 tokens 61 and 56), nor
+// for more ranks (1024 tokens 768 -> 2048 f32 rank 64 66 and 59).
+bool reads_across(const k82_lora_grad& p) { return p.dtype == K82_F32 && p.rank <= 16; }
 struct Layout { int64_t g, at, bt, scale, part, end; };         // bytes
 Layout layout(const k82_lora_grad& p, const k82_segments& s) {
-    const int64_t size = p.dtype == K82_F32 ? 4 : 2, used = std::min<int64_t>(s.n, p.adapters), all = (int64_t)p.cin + p.cout;
+    const int64_t size = p.dtype == K82_F32 ? 4 : 2, used = reads_across(p) ? 0 : std::min<int64_t>(s.n, p.adapters), all = (int64_t)p.cin + p.cout;
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
     Layout l;
     l.g = 0;
@@ -829,39 +859,39 @@ template <class T> hipError_t backward(const k82_lora_grad& p, const k82_segment
     char* w = (char*)ws;
     float *g = (float*)(w + l.g), *scale = (float*)(w + l.scale), *part = (float*)(w + l.part);
     T *at = (T*)(w + l.at), *bt = (T*)(w + l.bt);
-    // the adapters in use, numbered in the order of their index
-    std::vector<int> used, number(p.adapters, -1), first;
-    for (const RunTable& t : plan.tables) {
-        first.push_back((int)used.size());
-        for (int i = 0; i < t.runs; ++i) {
-            if (number[t.index[i]] < 0) { number[t.index[i]] = (int)used.size(); used.push_back(t.index[i]); }
-            else first.back() = number[t.index[i]];              // a run that the table before began
-        }
-    }
-    const int64_t factor = (int64_t)p.rank;
-    for (size_t i = 0; i < used.size(); i += op::kSegs) {
-        Used u;
-        u.n = (int)std::min<size_t>(op::kSegs, used.size() - i);
-        std::copy_n(used.begin() + i, u.n, u.index);
-        OP_TRY(op::run(lora_transpose_kernel<T>, dim3((p.cin + 31) / 32 + (p.cout + 31) / 32, (p.rank + 31) / 32, u.n), dim3(256), 0, st, u, p,
-                       at + i * factor * p.cin, bt + i * factor * p.cout, scale + i));
-    }
     std::vector<op::Seg> segs = op::merged(s);
-    for (op::Seg& v : segs)
-        if (v.index >= 0) v.index = number[v.index];
-    const k82_lora f{p.dtype, K82_ROWS, K82_ACT_NONE, p.cout, p.cin, p.rank, (int)used.size(), p.tokens, p.dy, p.lddy,
-                     p.dx_base, p.lddx_base, p.dx, p.lddx, bt, at, scale, g};
-    OP_TRY(forward<T>(f, segs, st));
+    if (reads_across(p)) {
+        const k82_lora f{p.dtype, K82_ROWS, K82_ACT_NONE, p.cout, p.cin, p.rank, p.adapters, p.tokens, p.dy, p.lddy,
+                         p.dx_base, p.lddx_base, p.dx, p.lddx, p.b, p.a, p.scale, g};
+        OP_TRY(forward<T>(f, segs, st, true));
+    } else {
+        // the adapters in use, numbered in the order of their index
+        std::vector<int> used, number(p.adapters, -1);
+        for (const RunTable& t : plan.tables)
+            for (int i = 0; i < t.runs; ++i)
+                if (number[t.index[i]] < 0) { number[t.index[i]] = (int)used.size(); used.push_back(t.index[i]); }
+        const int64_t factor = (int64_t)p.rank;
+        for (size_t i = 0; i < used.size(); i += op::kSegs) {
+            Used u;
+            u.n = (int)std::min<size_t>(op::kSegs, used.size() - i);
+            std::copy_n(used.begin() + i, u.n, u.index);
+            OP_TRY(op::run(lora_transpose_kernel<T>, dim3((p.cin + 31) / 32 + (p.cout + 31) / 32, (p.rank + 31) / 32, u.n), dim3(256), 0, st, u, p,
+                           at + i * factor * p.cin, bt + i * factor * p.cout, scale + i));
+        }
+        for (op::Seg& v : segs)
+            if (v.index >= 0) v.index = number[v.index];
+        const k82_lora f{p.dtype, K82_ROWS, K82_ACT_NONE, p.cout, p.cin, p.rank, (int)used.size(), p.tokens, p.dy, p.lddy,
+                         p.dx_base, p.lddx_base, p.dx, p.lddx, bt, at, scale, g};
+        OP_TRY(forward<T>(f, segs, st));
+    }
     const bool even = p.cin % Vec<T>::N == 0 && p.cout % Vec<T>::N == 0;
-    for (size_t i = 0; i < plan.tables.size(); ++i) {
-        const RunTable& t = plan.tables[i];
+    for (const RunTable& t : plan.tables) {
         const auto kernel = p.rank <= 16 ? (even ? lora_weight_kernel<T, 1, true> : lora_weight_kernel<T, 1, false>)
                                          : (even ? lora_weight_kernel<T, 2, true> : lora_weight_kernel<T, 2, false>);
-        OP_TRY(op::run(kernel, dim3(weight_groups(p), t.chunk0[t.runs] - t.chunk0[0]), dim3(64 * kWaves), 0, st, t, p, (const float*)g,
-                       (const float*)scale, first[i], part));
+        OP_TRY(op::run(kernel, dim3(weight_groups(p), t.chunk0[t.runs] - t.chunk0[0]), dim3(64 * kWaves), 0, st, t, p, (const float*)g, part));
     }
     for (const ReduceTable& t : plan.reduce)
-        OP_TRY(op::run(lora_reduce_kernel, dim3((p.cin + 63) / 64 + (p.cout + 63) / 64, (p.rank + 15) / 16, t.n), dim3(256), 0, st, t, p.cin, p.cout, p.rank,
+        OP_TRY(op::run(lora_reduce_kernel, dim3((p.cin + 63) / 64 + (p.cout + 63) / 64, (p.rank + 15) / 16, t.n), dim3(1024), 0, st, t, p.cin, p.cout, p.rank,
                        (const float*)part, p.da, p.db));
     return hipSuccess;
 }
