@@ -387,8 +387,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
 }
 
 // Channel-first: the same products, TT consecutive tokens a lane (tile t of a lane's tokens is TT col + t), 16 TT tokens a
-// workgroup, on the token grid of the tensor.  A tile that holds several segments is walked once for each; what is loaded of
-// the others' tokens stays in its own columns and is not stored.
+// workgroup, on the token grid of the tensor.  A tile that holds several segments has a workgroup for each (one that
+// walked them took twice as long as the others, and the launch as long as it: 16411 x 768
+// in 64 sentences 48 us, now 42); what is loaded of the others' tokens
+// stays in its own columns and is not stored.
 // The last tile reads at the tensor's end (t = its last pair, or token) and takes what is left: `second` where that pair is one
 // token ahead of the lane's.  at: bytes of the row
 template <int TT> __device__ __forceinline__ void load_tokens(float (&v)[TT], const char* base, uint32_t at, bool second) {
@@ -405,8 +407,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
     __shared__ __align__(16) char lds[most(NW * RT * 1024, NW * RT * TT * 1024)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     raw4* own = (raw4*)lds + wave * RT * 64;
-    const int first = sg.start[0], tokens = (int)p.tokens, c4 = 4 * (lane & 3);
-    const int tile = first / (16 * TT) * (16 * TT) + (int)blockIdx.x * 16 * TT, t0 = tile + TT * col;
+    const int s = seg_of(sg, blockIdx.x), k = sg.index[s], lo = sg.start[s], hi = lo + sg.len[s];
+    if (k < 0 && p.act == K82_ACT_NONE && p.base == p.y && !p.h) return;
+    const int tokens = (int)p.tokens, c4 = 4 * (lane & 3);
+    const int tile = lo / (16 * TT) * (16 * TT) + ((int)blockIdx.x - sg.tile0[s]) * 16 * TT, t0 = tile + TT * col;
     const uint32_t tb = 4 * min(t0, tokens - TT);
     const bool second = t0 == tokens - 1;
     // the lane's four channels (4 g + i) of 16 from base on, n of them there; behind those any that is (EVEN: four at a time, so
@@ -418,136 +422,130 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
             else load_tokens<TT>(v[i], base, min(4 * g + i, n - 1) * (uint32_t)ld * 4 + tb, second);
         }
     };
-    int s = place(sg.tile0, max(tile, first) - first);
-    for (; s < sg.n && sg.start[s] < tile + 16 * TT; ++s) {
-        const int k = sg.index[s], lo = sg.start[s], hi = lo + sg.len[s];
-        if (k == K82_SKIP) continue;
-        if (k < 0 && p.act == K82_ACT_NONE && p.base == p.y && !p.h) continue;
-        const int blocks = (p.cout + 15) / 16, stride = NW * gridDim.y;
-        int blk = (int)blockIdx.y * NW + wave;
-        float base[4][TT];
-        raw4 fac[RT];
-        const char* bp = (const char*)p.b + (int64_t)max(k, 0) * p.cout * p.rank * 4;
-        auto fetch = [&](int blk) {
-            const int n = p.cout - 16 * blk;
-            if (p.base) {
-                const char* q = (const char*)p.base + (int64_t)16 * blk * p.ldbase * 4;
-                load_rows(base, q, p.ldbase, n);
-            }
-            if (k >= 0) {
-                const uint32_t at = (min(lane >> 2, n - 1) * (uint32_t)p.rank + c4) * 4;
-#pragma unroll
-                for (int r = 0; r < RT; ++r) fac[r] = grab<float, EVEN>(bp + (int64_t)16 * blk * p.rank * 4, at + 64 * r, p.rank - 16 * r - c4, (16 * r + c4) * 4);
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int t = 0; t < TT; ++t) base[i][t] = 0.f;
-        if (blk < blocks) fetch(blk);
-        Second<float, RT> h[TT];
-        if (k >= 0) {
-            f4 acc[RT][TT];
-            uint32_t ao[RT];
-            const char* ap = (const char*)p.a + (int64_t)k * p.rank * p.cin * 4;
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                ao[r] = (min(16 * r + (lane >> 2), p.rank - 1) * (uint32_t)p.cin + c4) * 4;
-#pragma unroll
-                for (int t = 0; t < TT; ++t) acc[r][t] = f4{0.f, 0.f, 0.f, 0.f};
-            }
-            auto multiply = [&](const raw4 (&fa)[RT], const float (&fx)[4][TT]) {
-#pragma unroll
-                for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fa[r]);
-                wave_fence();
-                raw4 ta[RT];
-#pragma unroll
-                for (int r = 0; r < RT; ++r) ta[r] = get_tile(own + r * 64);
-                wave_fence();
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int t = 0; t < TT; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ta[r][i]), fx[i][t], acc[r][t], 0, 0, 0);
-            };
-            auto steps = [&](int i0, auto n) {                   // 16 channels a step: 4 g + i in instruction i
-                constexpr int n_ = decltype(n)::value;
-                float fx[n_][4][TT];
-                raw4 fa[n_][RT];
-#pragma unroll
-                for (int u = 0; u < n_; ++u) {
-                    const int c0 = 16 * (i0 + u * NW);
-                    const char* q = (const char*)p.x + (int64_t)c0 * p.ldx * 4;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) load_tokens<TT>(fx[u][i], q + (int64_t)i * p.ldx * 4, 4 * g * (uint32_t)p.ldx * 4 + tb, second);
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) fa[u][r] = load16(ap + 4 * c0, ao[r]);
-                }
-#pragma unroll
-                for (int u = 0; u < n_; ++u) multiply(fa[u], fx[u]);
-            };
-            const int full = p.cin / 16;
-            int i = wave;
-            for (; i + (U - 1) * NW < full; i += U * NW) steps(i, std::integral_constant<int, U>());
-            if (i < full) { steps(i, std::integral_constant<int, 1>()); i += NW; }
-            if (i == full && p.cin % 16) {                       // one wave: the last channels, zeros behind them
-                const int c0 = 16 * full, n = p.cin - c0;
-                const char* q = (const char*)p.x + (int64_t)c0 * p.ldx * 4;
-                raw4 fa[RT];
-                float fx[4][TT];
-#pragma unroll
-                for (int r = 0; r < RT; ++r) fa[r] = grab<float, EVEN>(ap + 4 * c0, ao[r], n - c4, 4 * c4);
-                load_rows(fx, q, p.ldx, n);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int t = 0; t < TT; ++t) fx[i][t] = 4 * g + i < n ? fx[i][t] : 0.f;
-                multiply(fa, fx);
-            }
-            int64_t tok[TT];
-            bool in[TT];
-#pragma unroll
-            for (int t = 0; t < TT; ++t) { tok[t] = t0 + t; in[t] = t0 + t >= lo && t0 + t < hi; }
-            join<float, NW, RT, TT>((f4(*)[RT * TT][64])lds, acc, h, p.rank, p.scale[k], blockIdx.y == 0 ? p.h : nullptr, tok, in);
-        } else if (p.h && blockIdx.y == 0) {
-            const int from = max(tile, lo), n = (min(tile + 16 * TT, hi) - from) * p.rank;
-            for (int i = threadIdx.x; i < n; i += 64 * NW) p.h[(int64_t)from * p.rank + i] = 0.f;
+    const int blocks = (p.cout + 15) / 16, stride = NW * gridDim.y;
+    int blk = (int)blockIdx.y * NW + wave;
+    float base[4][TT];
+    raw4 fac[RT];
+    const char* bp = (const char*)p.b + (int64_t)max(k, 0) * p.cout * p.rank * 4;
+    auto fetch = [&](int blk) {
+        const int n = p.cout - 16 * blk;
+        if (p.base) {
+            const char* q = (const char*)p.base + (int64_t)16 * blk * p.ldbase * 4;
+            load_rows(base, q, p.ldbase, n);
         }
-        for (; blk < blocks; blk += stride) {
-            f4 d[TT];
+        if (k >= 0) {
+            const uint32_t at = (min(lane >> 2, n - 1) * (uint32_t)p.rank + c4) * 4;
 #pragma unroll
-            for (int t = 0; t < TT; ++t) d[t] = f4{base[0][t], base[1][t], base[2][t], base[3][t]};
-            raw4 fb[RT];
-            if (k >= 0) {
+            for (int r = 0; r < RT; ++r) fac[r] = grab<float, EVEN>(bp + (int64_t)16 * blk * p.rank * 4, at + 64 * r, p.rank - 16 * r - c4, (16 * r + c4) * 4);
+        }
+    };
 #pragma unroll
-                for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fac[r]);
-                wave_fence();
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) fb[r] = get_tile(own + r * 64);
-                wave_fence();
+        for (int t = 0; t < TT; ++t) base[i][t] = 0.f;
+    if (blk < blocks) fetch(blk);
+    Second<float, RT> h[TT];
+    if (k >= 0) {
+        f4 acc[RT][TT];
+        uint32_t ao[RT];
+        const char* ap = (const char*)p.a + (int64_t)k * p.rank * p.cin * 4;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            ao[r] = (min(16 * r + (lane >> 2), p.rank - 1) * (uint32_t)p.cin + c4) * 4;
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[r][t] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        auto multiply = [&](const raw4 (&fa)[RT], const float (&fx)[4][TT]) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fa[r]);
+            wave_fence();
+            raw4 ta[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) ta[r] = get_tile(own + r * 64);
+            wave_fence();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ta[r][i]), fx[i][t], acc[r][t], 0, 0, 0);
+        };
+        auto steps = [&](int i0, auto n) {                   // 16 channels a step: 4 g + i in instruction i
+            constexpr int n_ = decltype(n)::value;
+            float fx[n_][4][TT];
+            raw4 fa[n_][RT];
+#pragma unroll
+            for (int u = 0; u < n_; ++u) {
+                const int c0 = 16 * (i0 + u * NW);
+                const char* q = (const char*)p.x + (int64_t)c0 * p.ldx * 4;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) load_tokens<TT>(fx[u][i], q + (int64_t)i * p.ldx * 4, 4 * g * (uint32_t)p.ldx * 4 + tb, second);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) fa[u][r] = load16(ap + 4 * c0, ao[r]);
             }
-            if (blk + stride < blocks) fetch(blk + stride);      // the next block is on its way while this one is multiplied
-            if (k >= 0)
 #pragma unroll
-                for (int t = 0; t < TT; ++t) d[t] = h[t].times(fb, d[t]);
-            char* yb = (char*)p.y + (int64_t)16 * blk * p.ldy * 4;
+            for (int u = 0; u < n_; ++u) multiply(fa[u], fx[u]);
+        };
+        const int full = p.cin / 16;
+        int i = wave;
+        for (; i + (U - 1) * NW < full; i += U * NW) steps(i, std::integral_constant<int, U>());
+        if (i < full) { steps(i, std::integral_constant<int, 1>()); i += NW; }
+        if (i == full && p.cin % 16) {                       // one wave: the last channels, zeros behind them
+            const int c0 = 16 * full, n = p.cin - c0;
+            const char* q = (const char*)p.x + (int64_t)c0 * p.ldx * 4;
+            raw4 fa[RT];
+            float fx[4][TT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = 4 * g + i;
-                float v[TT];
+            for (int r = 0; r < RT; ++r) fa[r] = grab<float, EVEN>(ap + 4 * c0, ao[r], n - c4, 4 * c4);
+            load_rows(fx, q, p.ldx, n);
 #pragma unroll
-                for (int t = 0; t < TT; ++t) v[t] = p.act == K82_ACT_GELU_NEW ? op_gelu_new(d[t][i]) : d[t][i];
-                if (16 * blk + c >= p.cout) continue;
-                float* q = (float*)(yb + (int64_t)i * p.ldy * 4 + (4 * g * (uint32_t)p.ldy + t0) * 4);
-                if (t0 >= lo && t0 + TT <= hi) {
-                    if constexpr (TT == 2) *(f2_any*)q = f2_any{v[0], v[1]};
-                    else q[0] = v[0];
-                } else
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int t = 0; t < TT; ++t)
-                        if (t0 + t >= lo && t0 + t < hi) q[t] = v[t];
-            }
+                for (int t = 0; t < TT; ++t) fx[i][t] = 4 * g + i < n ? fx[i][t] : 0.f;
+            multiply(fa, fx);
+        }
+        int64_t tok[TT];
+        bool in[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) { tok[t] = t0 + t; in[t] = t0 + t >= lo && t0 + t < hi; }
+        join<float, NW, RT, TT>((f4(*)[RT * TT][64])lds, acc, h, p.rank, p.scale[k], blockIdx.y == 0 ? p.h : nullptr, tok, in);
+    } else if (p.h && blockIdx.y == 0) {
+        const int from = max(tile, lo), n = (min(tile + 16 * TT, hi) - from) * p.rank;
+        for (int i = threadIdx.x; i < n; i += 64 * NW) p.h[(int64_t)from * p.rank + i] = 0.f;
+    }
+    for (; blk < blocks; blk += stride) {
+        f4 d[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) d[t] = f4{base[0][t], base[1][t], base[2][t], base[3][t]};
+        raw4 fb[RT];
+        if (k >= 0) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) put_tile(own + r * 64, fac[r]);
+            wave_fence();
+#pragma unroll
+            for (int r = 0; r < RT; ++r) fb[r] = get_tile(own + r * 64);
+            wave_fence();
+        }
+        if (blk + stride < blocks) fetch(blk + stride);      // the next block is on its way while this one is multiplied
+        if (k >= 0)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) d[t] = h[t].times(fb, d[t]);
+        char* yb = (char*)p.y + (int64_t)16 * blk * p.ldy * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = 4 * g + i;
+            float v[TT];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) v[t] = p.act == K82_ACT_GELU_NEW ? op_gelu_new(d[t][i]) : d[t][i];
+            if (16 * blk + c >= p.cout) continue;
+            float* q = (float*)(yb + (int64_t)i * p.ldy * 4 + (4 * g * (uint32_t)p.ldy + t0) * 4);
+            if (t0 >= lo && t0 + TT <= hi) {
+                if constexpr (TT == 2) *(f2_any*)q = f2_any{v[0], v[1]};
+                else q[0] = v[0];
+            } else
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+                    if (t0 + t >= lo && t0 + t < hi) q[t] = v[t];
         }
     }
 }
@@ -794,8 +792,8 @@ template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::S
                 constexpr int NW = RT <= 2 ? 8 : 4;
                 auto go = [&](auto tt) -> hipError_t {
                     constexpr int TT = decltype(tt)::value;
-                    for (const SegTable& t : op::tables(segs, 1)) {
-                        const int first = t.start[0], last = first + t.tile0[t.n] - 1, tiles = last / (16 * TT) - first / (16 * TT) + 1;
+                    for (const SegTable& t : op::tables(segs, 16 * TT, true)) {
+                        const int tiles = t.tile0[t.n];
                         OP_TRY(op::run(even ? lora_cols_kernel<NW, RT, TT, true> : lora_cols_kernel<NW, RT, TT, false>,
                                        dim3(tiles, parts(tiles, p.cout, 16 * NW)), dim3(64 * NW), 0, st, t, p));
                     }
@@ -900,7 +898,7 @@ template <class T> hipError_t backward(const k82_lora_grad& p, const k82_segment
 namespace op {
 int64_t workspace(const k82_lora_grad& p, const k82_segments& s) { return layout(p, s).end; }
 hipError_t launch(const k82_lora& p, const k82_segments& s, hipStream_t st) {
-    const std::vector<Seg> segs = merged(s, p.layout == K82_COLS);
+    const std::vector<Seg> segs = merged(s);
     return p.dtype == K82_F32 ? forward<float>(p, segs, st) : forward<bf16_t>(p, segs, st);
 }
 hipError_t launch(const k82_lora_grad& p, const k82_segments& s, void* ws, hipStream_t st) {

@@ -24,8 +24,8 @@ struct Seg { int start, len, index; };
 
 // without the skipped segments, or (walked) with those between others: kernels that walk the token axis pass over them
 std::vector<Seg> merged(const k82_segments& s, bool walked = false);
-// tables of at most kSegs segments with `tile` tokens per tile
-std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile);
+// tables of at most kSegs segments with `tile` tokens per tile, which start with their segment or (grid) at multiples of `tile`
+std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile, bool grid = false);
 
 // The token sums of the backward passes: the pieces of one index lie side by side (a run), and a run is cut into chunks
 // of at most `rows` tokens, whatever the pieces they come from.  One workgroup sums a chunk, a second launch adds the

@@ -174,7 +174,7 @@ std::vector<Seg> merged(const k82_segments& s, bool walked) {
     while (!v.empty() && v.back().index == K82_SKIP) v.pop_back();
     return v;
 }
-std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile) {
+std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile, bool grid) {
     std::vector<SegTable> out;
     for (size_t i0 = 0; i0 < segs.size(); i0 += kSegs) {
         out.emplace_back();
@@ -185,7 +185,8 @@ std::vector<SegTable> tables(const std::vector<Seg>& segs, int tile) {
             if (i < t.n) {
                 const Seg& g = segs[i0 + i];
                 t.start[i] = g.start; t.len[i] = g.len; t.index[i] = g.index;
-                t.tile0[i + 1] = t.tile0[i] + (g.len - 1) / tile + 1;
+                const int before = grid ? g.start % tile : 0;
+                t.tile0[i + 1] = t.tile0[i] + (before + g.len - 1) / tile + 1;
             } else {
                 t.start[i] = 0; t.len[i] = 0; t.index[i] = -1;
                 t.tile0[i + 1] = t.tile0[t.n];
