@@ -388,9 +388,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(RT >= 8
 
 // Channel-first: the same products, TT consecutive tokens a lane (tile t of a lane's tokens is TT col + t), 16 TT tokens a
 // workgroup, on the token grid of the tensor.  A tile that holds several segments has a workgroup for each (one that
-// walked them took twice as long as the others, and the launch as long as it: 16411 x 768
-// in 64 sentences 48 us, now 42); what is loaded of the others' tokens
-// stays in its own columns and is not stored.
+// walked them took twice as long as the others, and the launch as long as it: 16411 x 768 in 64 sentences 48 us, now 42);
+// what is loaded of the others' tokens stays in its own columns and is not stored.
 // The last tile reads at the tensor's end (t = its last pair, or token) and takes what is left: `second` where that pair is one
 // token ahead of the lane's.  at: bytes of the row
 template <int TT> __device__ __forceinline__ void load_tokens(float (&v)[TT], const char* base, uint32_t at, bool second) {
@@ -727,9 +726,8 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
     }
 }
 // da, db: the chunks of an adapter, 64 channels x 16 ranks a workgroup.  Four shares of four waves take every fourth chunk in
-// order, and their sums join in order (4096 tokens of one adapter, 768 / 768 bf16 rank 8, 85 chunks:
-// the backward pass 48 us with one share, 29 with four).
-// db's ranks leave side by side.
+// order, and their sums join in order (4096 tokens of one adapter, 768 / 768 bf16 rank 8, 85 chunks: the backward pass 48 us
+// with one share, 29 with four).  db's ranks leave side by side.
 __global__ __launch_bounds__(1024) void lora_reduce_kernel(ReduceTable rt, int cin, int cout, int rank, const float* part, float* da, float* db) {
     __shared__ float tile[4][64][17];
     const int nx = (cin + 63) / 64, k = blockIdx.z, r0 = 16 * blockIdx.y;
@@ -776,7 +774,7 @@ template <class F> hipError_t by_rank(int rank, F&& f) {
     return f(std::integral_constant<int, 8>());
 }
 // Parts of the output channels: until there are two workgroups a CU, `wide` channels (a block for each wave) at least.  More
-// parts cost more first products than their balance gains: 16411 x 768 f32 channel-first 48 us, with up to 1100 workgroups 56.
+// parts cost more first products than their balance gains: 16411 x 768 f32 channel-first 42 us, with up to 1200 workgroups 45.
 int parts(int tiles, int cout, int wide) { return std::max(1, std::min((cout + wide - 1) / wide, 512 / std::max(1, tiles))); }
 
 // 64 tokens a workgroup instead of 32, once that leaves two workgroups a CU: the factors are read half as often, which counts
