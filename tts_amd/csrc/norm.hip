@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kThreads<W>) void norm_rows_kernel(SegTable sg, k82
 // every STEP-th channel, a wave's load covers 64 / Q channels.  Tiles lie on the token grid of the tensor, not of the
 // sentences: rows start on lines and a batch of short sentences fills its tiles; the gain row is picked by token where a tile
 // holds several sentences.  The shape goes by the channel count alone, so a token's bits do not depend on its batch.
-// 32 tokens are the 128 bytes of a line: 16411 x 768 with a residual 46 us (3.3 TB/s; token rows: 34 us); 64 tokens 51 us and
+// 32 tokens are the 128 bytes of a line: 16411 x 768 with a residual 47 us (3.2 TB/s; token rows: 34 us); 64 tokens 51 us and
 // 16 tokens 50 to 56 us.  All of a tile is loaded, then all of it stored, which two workgroups on a CU overlap only in part.
 constexpr int kColsMax = 4096;                 // channels that fit
 template <int Q, int NW, int NV> __global__ __launch_bounds__(64 * NW) void norm_cols_kernel(SegTable sg, k82_layernorm p) {
