@@ -600,9 +600,11 @@ __device__ __forceinline__ void split3(const float (&v)[8], raw4& hi, raw4& mid,
 // k of the product: f32 takes it as it lies (4 tokens an instruction), bf16 through the transpose in registers.
 // More than 32 ranks are shares of neighbouring workgroups (their sums would leave one wave a SIMD): the channels come from the
 // shared cache again, 65536 tokens 768 / 2048 rank 64 130 us, with the shares one after the other 173.
+// Two steps in flight where the registers of two waves a SIMD hold them (D): the backward pass of 65536 tokens 768 / 2048 rank 8
+// bf16 193 -> 178 us, 32768 tokens 768 / 768 f32 110 -> 98.
 template <class T, int RT, bool EVEN>
-__global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k82_lora_grad p, const float* gs, float* part) {
-    constexpr int V = Vec<T>::N, M = 8, S = sizeof(T);           // M: 16 x 16 tiles along the channels
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))) void lora_weight_kernel(RunTable rt, k82_lora_grad p, const float* gs, float* part) {
+    constexpr int V = Vec<T>::N, M = 8, S = sizeof(T), D = RT == 1 ? 2 : 1;          // M: 16 x 16 tiles along the channels
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int chunk = rt.chunk0[0] + (int)blockIdx.y, run = place(rt.chunk0, chunk);
     const int u0 = rt.run_cum[run] + (chunk - rt.chunk0[run]) * rt.rows, u1 = min(u0 + rt.rows, rt.run_cum[run + 1]);
@@ -632,6 +634,21 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
     uint32_t rank_at[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) rank_at[r] = min(r0 + 16 * r + col, p.rank - 1);
+    // the steps of N tokens of a piece: D of them in flight, each place loaded again as soon as its step is in the operands
+    auto ring = [&](auto size, int n, auto& load, auto& use) {
+        constexpr int N = decltype(size)::value;
+        int i = 0;
+#pragma unroll
+        for (int b = 0; b < D; ++b)
+            if (N * (b + 1) <= n) load(b, N * b, std::true_type());
+        for (; i + 2 * D * N <= n; i += D * N)
+#pragma unroll
+            for (int b = 0; b < D; ++b) use(b, i + (D + b) * N, std::true_type());
+#pragma unroll
+        for (int b = 0; b < 2 * D - 1; ++b)
+            if (i + N <= n) { use(b % D, i + D * N, std::false_type()); i += N; }
+        if (i < n) { load(0, i, std::false_type()); use(0, n, std::false_type()); }
+    };
     int piece = place(rt.cum, u0);
     for (int u = u0; u < u1; ++piece) {                          // the pieces of a chunk, each a run of neighbouring tokens
         const int stop = min(u1, rt.cum[piece + 1]);
@@ -641,71 +658,75 @@ __global__ __launch_bounds__(64 * kWaves) void lora_weight_kernel(RunTable rt, k
         const char* zp = z + t0 * ld * S;
         const float* vp = v + t0 * p.rank;
         if constexpr (V == 8) {
-            auto step = [&](int i, auto whole) {                 // 32 tokens, 8 g + j in a lane; not whole: zeros behind the n-th
+            raw4 raw[D][8];
+            float w[D][RT][8];
+            auto load = [&](int b, int i, auto whole) {          // 32 tokens, 8 g + j in a lane; not whole: zeros behind the n-th
                 constexpr bool WHOLE = decltype(whole)::value;
-                raw4 raw[8], zt[8];
                 const raw4 zero = {0u, 0u, 0u, 0u};
-                float w[RT][8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int t = i + 8 * g + j;
                     const int at = WHOLE ? i + j : min(i + j, n - 1);
                     const uint32_t row = WHOLE ? 8 * g : max(min(8 * g, n - 1 - at), 0);
-                    raw[j] = take(zp + (int64_t)at * ld * S, row * (uint32_t)ld * S, c0 + 8 * col);
+                    raw[b][j] = take(zp + (int64_t)at * ld * S, row * (uint32_t)ld * S, c0 + 8 * col);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) w[r][j] = *(const float*)((const char*)(vp + (int64_t)at * p.rank) + 4 * (row * p.rank + rank_at[r]));
+                    for (int r = 0; r < RT; ++r) w[b][r][j] = *(const float*)((const char*)(vp + (int64_t)at * p.rank) + 4 * (row * p.rank + rank_at[r]));
                     if constexpr (!WHOLE) {
-                        raw[j] = t < n ? raw[j] : zero;
+                        raw[b][j] = t < n ? raw[b][j] : zero;
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) w[r][j] = t < n ? w[r][j] : 0.f;
+                        for (int r = 0; r < RT; ++r) w[b][r][j] = t < n ? w[b][r][j] : 0.f;
                     }
                 }
-                transpose8(raw, zt);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            auto use = [&](int b, int next, auto sure) {
+                raw4 zt[8], w3[RT][3];
+                transpose8(raw[b], zt);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    raw4 w3[3];
-                    split3(w[r], w3[0], w3[1], w3[2]);
+                for (int r = 0; r < RT; ++r) split3(w[b][r], w3[r][0], w3[r][1], w3[r][2]);
+                if (decltype(sure)::value || next + 32 <= n) load(b, next, std::true_type());
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
 #pragma unroll
                     for (int m = 0; m < 8; ++m)
 #pragma unroll
-                        for (int q = 2; q >= 0; --q) acc[m][r] = product<T>(zt[m], w3[q], acc[m][r]);
-                }
+                        for (int q = 2; q >= 0; --q) acc[m][r] = product<T>(zt[m], w3[r][q], acc[m][r]);
             };
-            int i = 0;
-            for (; i + 32 <= n; i += 32) step(i, std::true_type());
-            if (i < n) step(i, std::false_type());
+            ring(std::integral_constant<int, 32>(), n, load, use);
         } else {
-            auto step = [&](int i, auto whole) {                 // 16 tokens, 4 j + g in instruction j
+            raw4 raw[D][4][2];
+            float w[D][RT][4];
+            auto load = [&](int b, int i, auto whole) {          // 16 tokens, 4 j + g in instruction j
                 constexpr bool WHOLE = decltype(whole)::value;
-                raw4 raw[4][2];
                 const raw4 zero = {0u, 0u, 0u, 0u};
-                float w[RT][4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int t = i + 4 * j + g, at = WHOLE ? i + 4 * j : min(i + 4 * j, n - 1);
                     const uint32_t row = WHOLE ? g : max(min(g, n - 1 - at), 0);
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) raw[j][m] = take(zp + (int64_t)at * ld * S, row * (uint32_t)ld * S, c0 + 64 * m + 4 * col);
+                    for (int m = 0; m < 2; ++m) raw[b][j][m] = take(zp + (int64_t)at * ld * S, row * (uint32_t)ld * S, c0 + 64 * m + 4 * col);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) w[r][j] = *(const float*)((const char*)(vp + (int64_t)at * p.rank) + 4 * (row * p.rank + rank_at[r]));
+                    for (int r = 0; r < RT; ++r) w[b][r][j] = *(const float*)((const char*)(vp + (int64_t)at * p.rank) + 4 * (row * p.rank + rank_at[r]));
                     if constexpr (!WHOLE) {
 #pragma unroll
-                        for (int m = 0; m < 2; ++m) raw[j][m] = t < n ? raw[j][m] : zero;
+                        for (int m = 0; m < 2; ++m) raw[b][j][m] = t < n ? raw[b][j][m] : zero;
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) w[r][j] = t < n ? w[r][j] : 0.f;
+                        for (int r = 0; r < RT; ++r) w[b][r][j] = t < n ? w[b][r][j] : 0.f;
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            auto use = [&](int b, int next, auto sure) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int r = 0; r < RT; ++r)
 #pragma unroll
                         for (int m = 0; m < 8; ++m)
-                            acc[m][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw[j][m >> 2][m & 3]), w[r][j], acc[m][r], 0, 0, 0);
+                            acc[m][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw[b][j][m >> 2][m & 3]), w[b][r][j], acc[m][r], 0, 0, 0);
+                if (decltype(sure)::value || next + 16 <= n) load(b, next, std::true_type());
             };
-            int i = 0;
-            for (; i + 16 <= n; i += 16) step(i, std::true_type());
-            if (i < n) step(i, std::false_type());
+            ring(std::integral_constant<int, 16>(), n, load, use);
         }
     }
     // row 4 g + i of tile m is the channel 8 (4 g + i) + m (bf16) or 64 (m / 4) + 4 (4 g + i) + m % 4 (f32)
