@@ -846,11 +846,12 @@ int weight_groups(const k82_lora_grad& p) {
     const int shares = (p.rank + 31) / 32, pair = shares > 1 ? 2 : 1, per = kWaves / pair;
     return ((p.cin + 127) / 128 + (p.cout + 127) / 128 + per - 1) / per * ((shares + pair - 1) / pair);
 }
-// Tokens of a chunk of it: two (rank > 16: three, all that fit) workgroups a CU once there are tokens for them; more would not
-// run at once and their partial sums are traffic (65536 tokens 768 / 2048 rank 16: 512 workgroups 204 us for the whole
-// backward pass, 768 213 us).
+// Tokens of a chunk of it: as many workgroups a CU as its registers let run at once, two (f32 of more than 16 ranks: three),
+// once there are tokens for them; more would wait for them, and their partial sums are traffic.  The whole backward pass of
+// 65536 tokens 768 / 2048 bf16 rank 16: 512 workgroups 188 us, 768 196; 32768 tokens 768 / 768 bf16 rank 64 79 and 100; 65536
+// tokens 768 / 2048 f32 rank 32 443 and 396.
 int chunk_rows(const k82_lora_grad& p, int64_t tokens) {
-    const int64_t chunks = std::max<int64_t>(1, (p.rank <= 16 ? 512 : 768) / weight_groups(p));
+    const int64_t chunks = std::max<int64_t>(1, (p.rank <= 16 || p.dtype == K82_BF16 ? 512 : 768) / weight_groups(p));
     return (int)std::max<int64_t>(32, ((tokens + chunks - 1) / chunks + 31) / 32 * 32);
 }
 // One rank tile in f32: the factors are read across instead of being transposed first, a launch less (211 tokens 768 -> 768 rank
