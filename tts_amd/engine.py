@@ -78,13 +78,14 @@ class Engine(Operators):
         child._pending = None
         child.config, child.device = self.config, self.device
         child._parent = self
-        child._adapters = dict(getattr(self, "_adapters", {}))
         child._forks = []
         child.h = C.c_void_p()
         with self._lock:
             rc = self.lib.k82_fork(self.h, C.byref(child.h))
             if rc != 0:
                 raise RuntimeError(f"k82_fork failed ({rc}): {self.lib.k82_last_error(None).decode()}")
+            # under the same lock as the copy that k82_fork takes of the adapters: a name means the index it had at that moment
+            child._adapters = dict(getattr(self, "_adapters", {}))
             child.precision = self.precision
             self._forks.append(child)
         return child
