@@ -73,3 +73,40 @@ def test_a_fork_takes_names_and_table_of_one_moment(then):
             with pytest.raises(KeyError, match="not found"):
                 child._adapter_indices([n], 1)
     assert np.array_equal(child._adapter_indices([None], 1), [-1])
+
+
+@pytest.mark.parametrize("call", ["op_lora", "op_lora_grad", "op_layernorm", "op_layernorm_grad"])
+def test_a_first_call_beside_a_first_call(call):
+    """Whatever of a fresh handle the first call has set up so far, another thread's call goes through to the library (which
+    refuses it here: there is no handle behind this face)."""
+    import ctypes as C
+
+    import torch
+
+    from tts_amd import Operators, _lib
+    x, norm, one = torch.zeros(4, 8), torch.ones(1, 8), torch.ones(4)
+    a, b, scale, h, dy = torch.zeros(1, 2, 8), torch.zeros(1, 6, 2), torch.ones(1), torch.zeros(4, 2), torch.zeros(4, 6)
+    args = {"op_lora": (x, a, b, scale), "op_lora_grad": (x, dy, h, a, b, scale), "op_layernorm": (x, norm, norm),
+            "op_layernorm_grad": (x, x, norm, one, one)}[call]
+    said = []
+
+    def other(face):
+        try:
+            getattr(face, call)(*args)
+        except Exception as e:
+            said.append(repr(e))
+
+    class Face(Operators):
+        watched = threading.get_ident()
+
+        def __setattr__(self, name, value):
+            super().__setattr__(name, value)
+            if threading.get_ident() == self.watched and name not in ("device", "h", "lib"):
+                t = threading.Thread(target=other, args=(self,))
+                t.start()
+                t.join(60)
+
+    face = Face.__new__(Face)
+    face.device, face.h, face.lib = -1, C.c_void_p(), _lib.load()
+    other(face)
+    assert len(said) > 1 and all("k82 error -22" in s for s in said), said

@@ -121,17 +121,18 @@ class Operators:
     def _bind(self):
         """What every call needs: torch (never imported before a handle is) and the entry points for packed arguments."""
         import torch
-        self._torch = torch
         # the handle alone where torch offers it: a Stream object costs a microsecond
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
         self._codes = {torch.float32: 0, torch.bfloat16: 1}
         vp, i64 = C.c_void_p, C.c_int64
         forward, backward = C.CFUNCTYPE(C.c_int, vp, C.c_char_p, vp, vp), C.CFUNCTYPE(C.c_int, vp, C.c_char_p, vp, vp, i64, vp)
         size = C.CFUNCTYPE(i64, C.c_char_p, vp)
-        self._fn = {}
+        fn = {}
         for op in ("lora", "layernorm"):
-            self._fn[op] = forward((f"k82_op_{op}", self.lib))
-            self._fn[op + "_grad"] = (backward((f"k82_op_{op}_grad", self.lib)), size((f"k82_op_{op}_grad_workspace", self.lib)))
+            fn[op] = forward((f"k82_op_{op}", self.lib))
+            fn[op + "_grad"] = (backward((f"k82_op_{op}_grad", self.lib)), size((f"k82_op_{op}_grad_workspace", self.lib)))
+        self._fn = fn
+        self._torch = torch                                      # last: a thread that finds it set finds the rest
         return torch
 
     def _stream(self):
