@@ -99,6 +99,9 @@ def test_a_first_call_beside_a_first_call(call):
     class Face(Operators):
         watched = threading.get_ident()
 
+        def _stream(self):                                       # (torch has none to name without a GPU)
+            return 1
+
         def __setattr__(self, name, value):
             super().__setattr__(name, value)
             if threading.get_ident() == self.watched and name not in ("device", "h", "lib"):
