@@ -1,0 +1,66 @@
+"""The operators at the edges of what their arguments allow.  Tolerances: the bounds of test_gpu_operators.py, sums of
+roundings."""
+
+import pytest
+import torch
+
+from test_gpu_operators import TYPES, gen, lora_case, lora_grad_want, lora_want, ops, within  # noqa: F401
+from tts_amd import Segments
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------- values next to the largest
+def near_largest(dt, tokens, width):
+    """[tokens, width] and weights [1, width] of dt whose product is 2^127 (255/128 + 3/512) = 3.40e38, every term of it exact:
+    finite in 32 bits, half a step and more above the largest finite bf16 (255/128 2^127)."""
+    v, w = torch.zeros(tokens, width, device="cuda", dtype=dt), torch.zeros(1, width, device="cuda", dtype=dt)
+    v[:, 0], v[:, width - 1] = 2.0 ** 127, 2.0 ** 119
+    w[0, 0], w[0, width - 1] = 255 / 128, 1.5
+    v[1::2] *= -1
+    return v, w
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rank", [1, 7, 17, 40, 65])
+def test_a_large_finite_h_stays_finite(ops, dt, rank):
+    tokens, cin, cout = 37, 64, 72
+    x, w = near_largest(dt, tokens, cin)
+    _, base, _, b, _ = lora_case(tokens, cin, cout, rank, 2, dt, "dense", 5)
+    a = torch.zeros(2, rank, cin, device="cuda", dtype=dt)
+    a[:, rank - 1] = w
+    b = (b.float() * 2.0 ** -100).to(dt)
+    scale, seg = torch.ones(2, device="cuda"), Segments([0, 20, 37], [1, 0])
+    y, h = ops.op_lora(x, a, b, scale, seg, base=base, keep=True)
+    want, bound, h_want, h_bound = lora_want(x, base, a, b, scale, seg, "none")
+    assert h_want.abs().max() > torch.finfo(torch.bfloat16).max * 1.0015 and h_want.abs().max() < torch.finfo(torch.float32).max
+    within(h, h_want, h_bound + 1e-38, "h")
+    within(y, want, bound, "y")
+    assert want.abs().max() > 2.0 ** 14
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rank", [1, 7, 17, 40, 65])
+def test_large_finite_gradients_stay_finite(ops, dt, rank):
+    """dy B_k, and h, as the parts of the two products they enter: dx and da, and db."""
+    tokens, cin, cout = 37, 64, 72
+    seg = Segments([0, 20, 37], [1, 0])
+    scale = torch.ones(2, device="cuda")
+    x, _, a, _, _ = lora_case(tokens, cin, cout, rank, 2, dt, "dense", 6)
+    dy, w = near_largest(dt, tokens, cout)
+    b = torch.zeros(2, cout, rank, device="cuda", dtype=dt)
+    b[:, :, rank - 1] = w
+    x, a = (x.float() * 2.0 ** -100).to(dt), (a.float() * 2.0 ** -100).to(dt)
+    h = gen(7)(tokens, rank) * 2.0 ** -100
+    got = ops.op_lora_grad(x, dy, h, a, b, scale, seg)
+    for g, (want, bound), name in zip(got, lora_grad_want(x, dy, h, None, a, b, scale, seg), ("dx", "da", "db")):
+        within(g, want, bound + 1e-38, name)
+        assert want.abs().max() > 2.0 ** 10
+    # h next to the largest, dy small
+    x, dy, a, b, _ = lora_case(tokens, cin, cout, rank, 2, dt, "dense", 8)
+    dy = (dy.float() * 2.0 ** -100).to(dt)
+    h = torch.full((tokens, rank), (255 / 128 + 3 / 512) * 2.0 ** 127, device="cuda")
+    h[::3] *= -1
+    got = ops.op_lora_grad(x, dy, h, a, b, scale, seg)
+    for g, (want, bound), name in zip(got, lora_grad_want(x, dy, h, None, a, b, scale, seg), ("dx", "da", "db")):
+        within(g, want, bound + 1e-38, name)

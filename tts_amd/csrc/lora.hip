@@ -78,8 +78,10 @@ template <class T, int RT> __device__ __forceinline__ int rank_of(int tile, int 
     if constexpr (Vec<T>::N == 8 && RT > 1) return 32 * (tile >> 1) + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3);
     return 16 * tile + row;
 }
-// what a bf16 part leaves of v; nothing where the part is an infinity, which would make a NaN of the sum
-__device__ __forceinline__ float left_of(float v, float part) { return __builtin_isfinite(part) ? v - part : 0.f; }
+// v as far as a finite bf16 goes, and two of them as a part.  What is left behind a part is then a difference of finite numbers
+// where v is finite, also next to the largest f32, which alone would round to an infinity; where it is not, the last part is.
+__device__ __forceinline__ float in_bf16(float v) { return __builtin_amdgcn_fmed3f(v, -0x1.fep127f, 0x1.fep127f); }
+__device__ __forceinline__ uint32_t finite_pair(float a, float b) { return bf16_pair(in_bf16(a), in_bf16(b)); }
 // h as the second product's operand, and that product of one row tile of B with one tile of tokens.
 // f32: itself.  bf16: in two parts, h = hi + lo to 2^-16 (rounded to one part alone, h would cost half of the result's own
 // precision); at one tile both parts share an instruction, with B's four values twice.
@@ -103,8 +105,8 @@ template <int RT> struct Second<bf16_t, RT> {
     static __device__ __forceinline__ void parts(const f4& h, uint32_t* hi, uint32_t* lo) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            hi[j] = bf16_pair(h[2 * j], h[2 * j + 1]);
-            lo[j] = bf16_pair(left_of(h[2 * j], __uint_as_float(hi[j] << 16)), left_of(h[2 * j + 1], __uint_as_float(hi[j] & 0xffff0000u)));
+            hi[j] = finite_pair(h[2 * j], h[2 * j + 1]);
+            lo[j] = bf16_pair(h[2 * j] - __uint_as_float(hi[j] << 16), h[2 * j + 1] - __uint_as_float(hi[j] & 0xffff0000u));
         }
     }
     __device__ __forceinline__ void set(const f4 (&h)[RT]) {
@@ -588,10 +590,10 @@ __device__ __forceinline__ void split3(const float (&v)[8], raw4& hi, raw4& mid,
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float a = v[2 * j], b = v[2 * j + 1];
-        hi[j] = bf16_pair(a, b);
-        a = left_of(a, __uint_as_float(hi[j] << 16));
-        b = left_of(b, __uint_as_float(hi[j] & 0xffff0000u));
-        mid[j] = bf16_pair(a, b);
+        hi[j] = finite_pair(a, b);
+        a -= __uint_as_float(hi[j] << 16);
+        b -= __uint_as_float(hi[j] & 0xffff0000u);
+        mid[j] = finite_pair(a, b);
         lo[j] = bf16_pair(a - __uint_as_float(mid[j] << 16), b - __uint_as_float(mid[j] & 0xffff0000u));
     }
 }
