@@ -93,7 +93,9 @@ int k82_destroy(k82_handle* h);
  * replaces: the reference's two worker threads on one Kokoro object (epubviewer_06_latest_1_nov_2025_theme.py:407,692,715),
  * which onnxruntime serves with concurrent sess.run calls on one InferenceSession. */
 int k82_fork(k82_handle* parent, k82_handle** out);
-const char* k82_last_error(const k82_handle* h); /* h may be NULL: this thread's last error of a call without a handle (create, checks) */
+/* The text of the calling thread's last failed call on h (of any thread's, where this one had none); h may be NULL: of its last
+ * failed call without a handle (create, checks).  It stays as it is until the thread's next failure or k82_last_error. */
+const char* k82_last_error(const k82_handle* h);
 
 /* Weight upload.  `name` is "<submodule>.<state-dict key>" with weight-norm already folded
  * (e.g. "decoder.generator.ups.0.weight"), data is host f32 in PyTorch layout.  The layer

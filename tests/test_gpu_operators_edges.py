@@ -1,11 +1,12 @@
 """The operators at the edges of what their arguments allow.  Tolerances: the bounds of test_gpu_operators.py, sums of
 roundings."""
+import threading
 
 import pytest
 import torch
 
 from test_gpu_operators import TYPES, gen, lora_case, lora_grad_want, lora_want, ops, within  # noqa: F401
-from tts_amd import Segments
+from tts_amd import Segments, _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,54 @@ def test_large_finite_gradients_stay_finite(ops, dt, rank):
     got = ops.op_lora_grad(x, dy, h, a, b, scale, seg)
     for g, (want, bound), name in zip(got, lora_grad_want(x, dy, h, None, a, b, scale, seg), ("dx", "da", "db")):
         within(g, want, bound + 1e-38, name)
+
+
+# ---------------------------------------------------------------------------------------------- refusals on several threads
+def norm_args(eps):
+    x, gain, offset = (torch.ones(1, 8, device="cuda") for _ in range(3))
+    return _lib.K82Layernorm(0, 0, 8, 1, eps, 1, x.data_ptr(), 8, None, 0, x.data_ptr(), 8, gain.data_ptr(), offset.data_ptr(), None,
+                             None), (x, gain, offset)
+
+
+def test_a_refusal_keeps_its_reason_beside_another_threads(ops):
+    """The text of a thread's own last failed call on the handle; a thread that had none reads the handle's last."""
+    lib, seg, (bad, keep) = ops.lib, Segments([0, 1], [0]), norm_args(-1.0)
+    read = []
+
+    def other():
+        read.append(lib.k82_last_error(ops.h))
+        assert lib.k82_op_layernorm(ops.h, norm_args(1.0)[0], Segments([0, 1], [7]).c, None) == -22
+        read.append(lib.k82_last_error(ops.h))
+
+    assert lib.k82_op_layernorm(ops.h, bad, seg.c, None) == -22
+    t = threading.Thread(target=other)
+    t.start()
+    t.join(60)
+    assert b"eps" in lib.k82_last_error(ops.h)
+    assert b"eps" in read[0] and b"index 7" in read[1]
+    late = []
+    t = threading.Thread(target=lambda: late.append(lib.k82_last_error(ops.h)))
+    t.start()
+    t.join(60)
+    assert b"index 7" in late[0]
+
+
+def test_refusals_of_many_threads_at_once(ops):
+    wrong = []
+
+    def work(k):
+        for _ in range(300):
+            x = torch.ones(1, 8, device="cuda")
+            try:
+                ops.op_layernorm(x, x, x, Segments([0, 1], [100 + k]))
+                wrong.append("accepted")
+            except ValueError as e:
+                if f"index {100 + k} " not in str(e):
+                    wrong.append(str(e))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]

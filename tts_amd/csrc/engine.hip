@@ -37,6 +37,10 @@ struct K82Error : std::runtime_error {
 inline int ru(int a, int m) { return (a + m - 1) / m * m; }
 
 thread_local std::string g_create_error;      // k82_last_error(NULL): the calling thread's last create / check error
+// k82_last_error(h): the calling thread's last failed call on a handle.  Its text belongs to the thread, so no other thread's
+// failure replaces it while it is read.
+struct ThreadError { const k82_handle* h = nullptr; std::string text; };
+thread_local ThreadError g_thread_error;
 
 // ---- k82_pcm16_static: the one entry point that allocates nothing (include/k82.h) ------------------------------
 // Staging for host -> device -> host conversion lives in a file-scope device array instead of the workspace arena.
@@ -214,7 +218,13 @@ struct k82_handle : K82Weights {
     hipStream_t own_stream = nullptr;
     hipStream_t st = nullptr;          // stream of the current call
     std::mutex mu;
-    std::string err;
+    std::string err;                   // of the last failed call of any thread; err_mu, so that no reader waits for a running call
+    mutable std::mutex err_mu;
+    void failed(const std::string& what) {
+        g_thread_error = {this, what};
+        std::lock_guard<std::mutex> lk(err_mu);
+        err = what;
+    }
     bool finalized = false;
     std::unordered_map<std::string, HostT> host;
     std::vector<void*> wallocs;        // device weight allocations
@@ -1414,13 +1424,13 @@ template <class F> int guarded(k82_handle* h, void* stream, F&& f) {
         f();
         return K82_OK;
     } catch (const K82Error& e) {
-        h->err = e.what();
+        h->failed(e.what());
         return e.code;
     } catch (const std::bad_alloc&) {
-        h->err = "host allocation failed";
+        h->failed("host allocation failed");
         return K82_ENOMEM;
     } catch (const std::exception& e) {
-        h->err = e.what();
+        h->failed(e.what());
         return K82_EINVAL;
     }
 }
@@ -1472,6 +1482,7 @@ int k82_create(const k82_config* cfg, int device, k82_handle** out) {
     k82_handle* h = nullptr;
     try {
         h = new k82_handle();
+        if (g_thread_error.h == h) g_thread_error.h = nullptr;       // the memory of a handle that was
         h->cfg = *cfg;
         h->device = device;
         HIPCHK(hipSetDevice(device));
@@ -1503,6 +1514,7 @@ int k82_fork(k82_handle* parent, k82_handle** out) {
         REQUIRE(parent->finalized, K82_ESTATE, "k82_fork needs a finalized handle");
         REQUIRE(!parent->parent, K82_ESTATE, "k82_fork: fork the handle that owns the weights, not one of its forks");
         h = new k82_handle();
+        if (g_thread_error.h == h) g_thread_error.h = nullptr;
         h->cfg = parent->cfg;
         h->device = parent->device;
         HIPCHK(hipSetDevice(h->device));
@@ -1527,7 +1539,7 @@ int k82_fork(k82_handle* parent, k82_handle** out) {
         return K82_OK;
     } catch (const K82Error& e) {
         g_create_error = e.what();
-        parent->err = e.what();
+        parent->failed(e.what());
         if (h) { for (void* p : h->wallocs) (void)hipFree(p); if (h->own_stream) (void)hipStreamDestroy(h->own_stream); }
         delete h;
         return e.code;
@@ -1541,8 +1553,7 @@ int k82_fork(k82_handle* parent, k82_handle** out) {
 int k82_destroy(k82_handle* h) {
     if (!h) return K82_EINVAL;
     if (h->forks.load() > 0) {           // its forks read this handle's weights
-        std::lock_guard<std::mutex> lk(h->mu);
-        h->err = "k82_destroy: " + std::to_string(h->forks.load()) + " handle(s) made by k82_fork are still alive; destroy them first";
+        h->failed("k82_destroy: " + std::to_string(h->forks.load()) + " handle(s) made by k82_fork are still alive; destroy them first");
         return K82_ESTATE;
     }
     {
@@ -1561,7 +1572,14 @@ int k82_destroy(k82_handle* h) {
     return K82_OK;
 }
 
-const char* k82_last_error(const k82_handle* h) { return h ? h->err.c_str() : g_create_error.c_str(); }
+const char* k82_last_error(const k82_handle* h) {
+    if (!h) return g_create_error.c_str();
+    if (g_thread_error.h == h) return g_thread_error.text.c_str();
+    static thread_local std::string copy;      // another thread's: what the handle says now
+    std::lock_guard<std::mutex> lk(h->err_mu);
+    copy = h->err;
+    return copy.c_str();
+}
 
 int k82_set_tensor(k82_handle* h, const char* name, const float* data, const int64_t* shape, int ndim) {
     return guarded(h, nullptr, [&] {
