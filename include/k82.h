@@ -222,7 +222,7 @@ int k82_pcm16_static(k82_handle* h, const float* src, int16_t* dst, int64_t n, v
  * Layout of a tensor [tokens][channels]: K82_ROWS element (t, c) at p[t * ld + c], ld >= channels; K82_COLS, the
  * engine's own channel-first layout, at p[c * ld + t], ld >= tokens.  K82_COLS exists in K82_F32 only and in the forward
  * operators only.  All tensors of a call share dtype and layout unless stated; no alignment beyond the element's own is
- * needed.  At most 2^24 - 1 tokens, 2^20 channels and an ld of 2^25 a call.
+ * needed.  At most 2^24 - 1 tokens, 2^20 channels, an ld of 2^25 and, backward, 2^24 - 1 adapters or gains a call.
  *
  * Segments cut the token axis: segment s holds the tokens [off[s], off[s+1]), 0 <= off[0] <= ... <= off[n] <= tokens,
  * and uses adapter (gain) index[s]; an index may come any number of times and a segment may be empty.  K82_SKIP (the padding

@@ -101,6 +101,7 @@ std::string check(const k82_lora_grad* p, const k82_segments* s) {
     if (!p) return "arguments must not be NULL";
     OP_CHECK(check_sizes(p->dtype, K82_ROWS, p->tokens, {p->cin, p->cout}));
     OP_CHECK(check_lora_factors(p->rank, p->adapters, p->a, p->b, p->scale));
+    if (p->adapters >= 1 << 24) return "adapters must be less than 2^24";       // (each has sums to be written, by numbers of 32 bits)
     if (p->adapters > 0 && (!p->da || !p->db)) return "da and db must not be NULL";
     OP_CHECK(check_segments(s, p->tokens, -1, p->adapters, "adapters"));
     const int size = p->dtype == K82_F32 ? 4 : 2;
@@ -143,6 +144,7 @@ std::string check(const k82_layernorm_grad* p, const k82_segments* s) {
     if (!p) return "arguments must not be NULL";
     OP_CHECK(check_sizes(p->dtype, K82_ROWS, p->tokens, {p->c}));
     if (p->gains < 1 || !p->gain || !p->dgain || !p->doffset) return "gain, dgain and doffset must hold at least one row";
+    if (p->gains >= 1 << 24) return "gains must be less than 2^24";
     if (p->tokens > 0 && (!p->mean || !p->rstd)) return "mean and rstd must not be NULL";
     OP_CHECK(check_segments(s, p->tokens, 0, p->gains, "gains"));
     const int size = p->dtype == K82_F32 ? 4 : 2;
