@@ -5,7 +5,7 @@ import threading
 import pytest
 import torch
 
-from test_gpu_operators import TYPES, gen, lora_case, lora_grad_want, lora_want, ops, within  # noqa: F401
+from test_gpu_operators import TYPES, gen, lora_case, lora_grad_want, lora_want, norm_case, ops, within  # noqa: F401
 from tts_amd import Segments, _lib
 
 pytestmark = pytest.mark.gpu
@@ -116,3 +116,25 @@ def test_refusals_of_many_threads_at_once(ops):
     for t in threads:
         t.join()
     assert not wrong, wrong[:3]
+
+
+# ---------------------------------------------------------------------------------------------- the largest launches
+def test_layernorm_of_as_many_wide_rows_as_a_call_holds(ops):
+    """2^24 - 1 rows of 1024 threads each: equal rows give equal results, the first and the last of every part among them."""
+    tokens, c = (1 << 24) - 1, 4097
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    if free < 2 * tokens * c + (16 << 30):
+        pytest.skip(f"{free >> 30} GiB are free, 137 GB of rows and room to compare are needed")
+    row, _, gain, offset = norm_case(1, c, 1, torch.bfloat16, "dense", 3)
+    want = ops.op_layernorm(row, gain, offset)
+    assert not torch.equal(want, row)
+    x = torch.empty(tokens, c, device="cuda", dtype=torch.bfloat16)
+    try:
+        x.copy_(row.expand(tokens, c))
+        assert ops.op_layernorm(x, gain, offset, out=x) is x
+        for i in range(0, tokens, 1 << 20):
+            assert (x[i:i + (1 << 20)] == want).all(), i
+    finally:
+        del x
+        torch.cuda.empty_cache()

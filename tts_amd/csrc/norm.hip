@@ -445,8 +445,10 @@ template <class T> hipError_t forward(const k82_layernorm& p, const k82_segments
     }
     return by_width<T, kRowMax>(p.c, [&](auto w, auto nv) -> hipError_t {
         constexpr int W = decltype(w)::value, R = W == 1 ? 4 : 1;
-        // rows behind each other in a workgroup share the gain's registers, once there are rows for every CU
-        const int tile = R * (int)std::max<int64_t>(1, std::min<int64_t>(4, op::covered(s) / (R * 2048)));
+        // rows behind each other in a workgroup share the gain's registers, once there are rows for every CU (8 rather than 4 of
+        // the widest where 1024 threads for every four would reach the 2^32 that a launch cannot hold)
+        const int64_t tokens = op::covered(s), most = W == 16 && tokens >= 1 << 23 ? 8 : 4;
+        const int tile = R * (int)std::max<int64_t>(1, std::min(most, tokens / (R * 2048)));
         for (const SegTable& t : op::tables(segs, tile))
             OP_TRY(op::run(norm_rows_kernel<T, W, decltype(nv)::value>, dim3(t.tile0[t.n]), dim3(kThreads<W>), 0, st, t, p, tile));
         return hipSuccess;
