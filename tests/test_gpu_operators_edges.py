@@ -1,11 +1,13 @@
 """The operators at the edges of what their arguments allow.  Tolerances: the bounds of test_gpu_operators.py, sums of
 roundings."""
+import ctypes as C
 import threading
 
 import pytest
 import torch
 
-from test_gpu_operators import TYPES, gen, lora_case, lora_grad_want, lora_want, norm_case, ops, within  # noqa: F401
+from test_gpu_operators import (TYPES, cut, gen, lora_case, lora_grad_want, lora_want, norm_case, norm_grad_want, ops,  # noqa: F401
+                                tensor, within)
 from tts_amd import Segments, _lib
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +140,83 @@ def test_layernorm_of_as_many_wide_rows_as_a_call_holds(ops):
     finally:
         del x
         torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------------------- workspaces
+def in_poisoned_workspace(ops, op, p, seg):
+    """The C entry point with a workspace of exactly the bytes it asks for, every one 0xff (NaN in either type), and a guard
+    behind it that stays as it was."""
+    need = getattr(ops.lib, f"k82_op_{op}_workspace")(p, seg.c)
+    assert need > 0
+    ws = torch.full((need + 4096,), 0xff, device="cuda", dtype=torch.uint8)
+    guard = torch.arange(4096, device="cuda").to(torch.uint8)
+    ws[need:] = guard
+    assert ws.data_ptr() % 256 == 0
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream or 1)
+    call = getattr(ops.lib, f"k82_op_{op}")
+    assert call(ops.h, p, seg.c, ws.data_ptr(), need - 1, stream) == -28
+    assert call(ops.h, p, seg.c, ws.data_ptr(), need, stream) == 0, ops.lib.k82_last_error(ops.h)
+    assert torch.equal(ws[need:], guard)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("tokens,cin,cout,rank,adapters,segs", [
+    (1, 1, 1, 1, 1, 1), (2, 5, 3, 3, 2, 2), (63, 129, 65, 17, 2, 3), (64, 64, 64, 64, 1, 1), (211, 768, 768, 7, 1, 1),
+    (257, 200, 96, 128, 2, 5), (300, 96, 40, 7, 6, 290), (3000, 260, 513, 33, 3, 11), (700, 140, 70, 8, 400, 500),
+    (9000, 64, 100, 4, 2, 3), (34000, 136, 72, 40, 3, 7), (260, 24, 16, 4, 2, 258),
+])
+def test_lora_backward_writes_all_it_reads_of_its_workspace(ops, dt, tokens, cin, cout, rank, adapters, segs):
+    x, dy, a, b, scale = lora_case(tokens, cin, cout, rank, adapters, dt, "dense", tokens + 1)
+    seg = cut(tokens, segs, adapters, seed=tokens, none=segs > 1)
+    h = gen(3)(tokens, rank)
+    dx, da, db = (torch.full(s, float("nan"), device="cuda", dtype=t) for s, t in (((tokens, cin), dt), (a.shape, torch.float32),
+                                                                                  (b.shape, torch.float32)))
+    p = _lib.K82LoraGrad(TYPES.index(dt), cin, cout, rank, adapters, tokens, x.data_ptr(), cin, dy.data_ptr(), cout, h.data_ptr(),
+                         None, 0, dx.data_ptr(), cin, a.data_ptr(), b.data_ptr(), scale.data_ptr(), da.data_ptr(), db.data_ptr())
+    in_poisoned_workspace(ops, "lora_grad", p, seg)
+    for g, (want, bound), name in zip((dx, da, db), lora_grad_want(x, dy, h, None, a, b, scale, seg), ("dx", "da", "db")):
+        within(g, want, bound + 1e-38, name)
+    for g, again in zip((dx, da, db), ops.op_lora_grad(x, dy, h, a, b, scale, seg)):
+        assert torch.equal(g, again)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("tokens,c,gains,segs", [
+    (1, 1, 1, 1), (1, 768, 2, 1), (3, 2, 2, 2), (97, 513, 1, 1), (65, 768, 4, 9), (300, 130, 5, 290), (130, 1000, 2, 3), (9, 5000, 2, 2),
+    (6, 20011, 1, 1), (300, 9000, 3, 40), (4000, 96, 3, 8), (600, 40, 300, 400), (40000, 64, 2, 5),
+])
+def test_layernorm_backward_writes_all_it_reads_of_its_workspace(ops, dt, tokens, c, gains, segs):
+    x, res, gain, offset = norm_case(tokens, c, gains, dt, "dense", tokens + c)
+    dy = tensor(gen(5), tokens, c, dt, scale=0.1)
+    seg = cut(tokens, segs, gains, seed=c)
+    _, mean, rstd = ops.op_layernorm(x, gain, offset, seg, res=res, eps=1e-5, stats=True)
+    dx = torch.full((tokens, c), float("nan"), device="cuda", dtype=dt)
+    dgain, doffset = (torch.full((gains, c), float("nan"), device="cuda") for _ in range(2))
+    p = _lib.K82LayernormGrad(TYPES.index(dt), c, gains, tokens, x.data_ptr(), c, res.data_ptr(), c, dy.data_ptr(), c, dx.data_ptr(), c,
+                              gain.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dgain.data_ptr(), doffset.data_ptr())
+    in_poisoned_workspace(ops, "layernorm_grad", p, seg)
+    for g, (want, bound), name in zip((dx, dgain, doffset), norm_grad_want(x, res, dy, gain, mean, rstd, seg), ("dx", "dgain", "doffset")):
+        within(g, want, bound, name)
+    for g, again in zip((dx, dgain, doffset), ops.op_layernorm_grad(x, dy, gain, mean, rstd, seg, res=res)):
+        assert torch.equal(g, again)
+
+
+def test_a_workspace_that_covers_tokens_of_nobody(ops):
+    """The sizes go by the cut's ends, the sums by what lies between: padding, sentences without an adapter, unused ones."""
+    tokens, c, rank = 4000, 72, 9
+    x, dy, a, b, scale = lora_case(tokens, c, c, rank, 200, torch.bfloat16, "dense", 4)
+    seg = Segments.of_padded([(7 * i) % 41 for i in range(100)], [(3 * i) % 200 if i % 5 else -1 for i in range(100)], 40)
+    h = gen(4)(tokens, rank)
+    dx = torch.full((tokens, c), float("nan"), device="cuda", dtype=torch.bfloat16)
+    da, db = torch.full(a.shape, float("nan"), device="cuda"), torch.full(b.shape, float("nan"), device="cuda")
+    p = _lib.K82LoraGrad(1, c, c, rank, 200, tokens, x.data_ptr(), c, dy.data_ptr(), c, h.data_ptr(), None, 0, dx.data_ptr(), c,
+                         a.data_ptr(), b.data_ptr(), scale.data_ptr(), da.data_ptr(), db.data_ptr())
+    in_poisoned_workspace(ops, "lora_grad", p, seg)
+    rows = torch.cat([torch.arange(int(lo), int(hi)) for lo, hi, k in zip(seg.offsets[:-1], seg.offsets[1:], seg.index) if k >= -1]).cuda()
+    want = lora_grad_want(x, dy, h, None, a, b, scale, seg)
+    within(dx[rows], want[0][0][rows], want[0][1][rows], "dx")
+    within(da, want[1][0], want[1][1] + 1e-38, "da")
+    within(db, want[2][0], want[2][1] + 1e-38, "db")
+    left = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    left[rows] = False
+    assert torch.isnan(dx[left].float()).all()
