@@ -123,8 +123,8 @@ int k82_durations(k82_handle* h, const int64_t* ids, const int32_t* lens, int B,
                   int32_t* pred_dur, int64_t* n_frames, void* stream);
 
 /* Adapters of tuned voices: low-rank factors beside the Linears of the (layer-shared) ALBERT encoder and / or gains and offsets
- * in the place of its two layer norms.  Replaces the handle's adapters (n = 0: none); host f32, copied before the call
- * returns.  A fork (k82_fork) inherits what its parent holds; while forks live, and on a fork, the call is refused
+ * in the place of its two layer norms.  Replaces the handle's adapters (n = 0: none); host f32, all of it finite, copied before the
+ * call returns.  A fork (k82_fork) inherits what its parent holds; while forks live, and on a fork, the call is refused
  * (K82_ESTATE), since they read the same memory.  No counterpart in the reference, whose voices are style vectors only. */
 #define K82_ADAPTER_QUERY 0
 #define K82_ADAPTER_KEY 1

@@ -77,3 +77,15 @@ def test_samples_do_not_depend_on_the_batch(adapted):  # noqa: F811
     for i, (got, want) in enumerate(zip(batch, run(list(range(140)), None))):
         if names[i] is None:
             assert all(np.array_equal(u, v) for u, v in zip(got, want)), i
+
+
+def test_adapters_that_are_not_numbers_are_refused_by_the_library(adapted):  # noqa: F811
+    voice = make_adapter(rank=3, seed=5)
+    adapted.set_adapters({"x": voice})
+    for values in (*voice.factors["ffn_output"], *voice.norms["attention_norm"]):
+        kept, values.flat[-1] = float(values.flat[-1]), float("nan")
+        with pytest.raises(ValueError, match="must be finite"):
+            adapted.set_adapters({"y": voice})
+        values.flat[-1] = kept
+    assert adapted._adapter_indices(["x"], 1).tolist() == [0]                         # the set is what it was
+    adapted.set_adapters({"y": voice})

@@ -41,6 +41,8 @@ class Adapter:
             if a.shape != (rank, cin) or b.shape != (cout, rank) or not 1 <= rank <= 128:
                 raise ValueError(f"Adapter: {part} needs a [rank, {cin}] and b [{cout}, rank] with rank 1 to 128, "
                                  f"got {a.shape} and {b.shape}")
+            if not (np.isfinite(a).all() and np.isfinite(b).all()):
+                raise ValueError(f"Adapter: the factors of {part} must be finite")
             if self.rank not in (0, rank):
                 raise ValueError(f"Adapter: one rank for all parts, got {self.rank} and {rank}")
             self.rank = rank
@@ -51,6 +53,8 @@ class Adapter:
             gain, offset = (np.ascontiguousarray(v, dtype=np.float32) for v in pair)
             if gain.shape != (d,) or offset.shape != (d,):
                 raise ValueError(f"Adapter: {norm} needs a gain and an offset of {d} values")
+            if not (np.isfinite(gain).all() and np.isfinite(offset).all()):
+                raise ValueError(f"Adapter: gain and offset of {norm} must be finite")
             self.norms[norm] = (gain, offset)
 
     @classmethod

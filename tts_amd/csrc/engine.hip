@@ -935,6 +935,17 @@ struct k82_handle : K82Weights {
             REQUIRE(!any || (v[i].rank >= 1 && v[i].rank <= K82_LORA_MAX_RANK), K82_EINVAL, "adapter " + std::to_string(i) + ": rank must be in [1, 128]");
             REQUIRE(!any || std::isfinite(v[i].scale), K82_EINVAL, "adapter " + std::to_string(i) + ": scale must be finite");
             if (any) t.rank = std::max(t.rank, v[i].rank);
+            // (one value that is none would reach every duration of its sentence, whose batch then fails as a whole)
+            bool finite = true;
+            auto look = [&](const float* q, size_t k) { for (size_t j = 0; q && j < k; ++j) finite &= std::isfinite(q[j]); };
+            for (int p = 0; p < K82_ADAPTER_PARTS; ++p) {
+                int cin, cout;
+                adapter_dims(cfg, p, &cin, &cout);
+                look(v[i].a[p], (size_t)v[i].rank * cin);
+                look(v[i].b[p], (size_t)v[i].rank * cout);
+            }
+            for (int m = 0; m < 2; ++m) { look(v[i].gain[m], cfg.bert_hidden); look(v[i].offset[m], cfg.bert_hidden); }
+            REQUIRE(finite, K82_EINVAL, "adapter " + std::to_string(i) + ": factors, gains and offsets must be finite");
         }
         t.rank = ru(t.rank, 4);                // whole 16-byte loads
         std::vector<float> all;                // the image of one allocation
