@@ -144,7 +144,8 @@ typedef struct k82_adapter {
 int k82_set_adapters(k82_handle* h, const k82_adapter* adapters, int32_t n);
 
 /* k82_durations with an adapter for each sentence: adapter[b] in [-1, n), host i32[B]; -1 (and NULL for all) is the model as
- * it is.  A sentence gives the same bits whatever the adapters of the others in its batch. */
+ * it is.  A sentence gives the same bits whatever the adapters of the others in its batch.  (All adapters of a set run at the
+ * largest rank of the set, and the order of sums goes by that rank's tiles: in another set a voice may differ in roundings.) */
 int k82_durations_adapted(k82_handle* h, const int64_t* ids, const int32_t* lens, int B, int Tmax, const float* ref_s,
                           const float* speed, const int32_t* forced_dur, const int32_t* adapter, int32_t* pred_dur,
                           int64_t* n_frames, void* stream);
@@ -247,7 +248,8 @@ typedef struct k82_segments {
 
 /* y = act(base + scale[k] * (x A_k^T) B_k^T), k = index of the token's segment; k = -1 (no adapter): y = act(base).
  * base is what the shared projection wrote (NULL: 0) and may be y itself; x and y must not overlap.  Products of 16-bit
- * operands are exact, all sums are 32 bits wide, and y is rounded once.
+ * operands are exact, all sums are 32 bits wide, and y is rounded once; with K82_BF16, x A_k^T enters the second product in two
+ * 16-bit parts, to 2^-16 of its value.
  * h (NULL: not kept): f32[tokens][rank], x A_k^T (0 where k = -1), which k82_op_lora_grad takes. */
 typedef struct k82_lora {
     int32_t dtype, layout, act;
@@ -267,8 +269,9 @@ int k82_op_lora(k82_handle* h, const k82_lora* p, const k82_segments* seg, void*
  *   dx = dx_base + scale[k] (dy B_k) A_k   (k = -1: dx = dx_base; dx_base NULL: 0; dx_base may be dx itself)
  *   da_k = scale[k] sum_t (dy B_k)^T x,  db_k = scale[k] sum_t dy^T h   (f32; zero for an adapter without tokens)
  * Sums over tokens are taken in a fixed order: the same call gives the same bits.  dx may not overlap x or dy.
- * K82_BF16 takes h and dy B_k in parts, in the forward call too: an infinity of x, dy or a factor that meets them gives an
- * infinity or a NaN, never a finite number.
+ * K82_BF16 takes h and dy B_k in parts, in the forward call too (two for dx, three, 2^-24 of the value, for da and db): an infinity
+ * of x, dy or a factor that meets them gives an infinity or a NaN, never a finite number.  A finite h or
+ * dy B_k stays finite in its parts.
  * workspace: device memory of at least k82_op_lora_grad_workspace bytes, 256-byte aligned, the caller's until the
  * enqueued work is done. */
 typedef struct k82_lora_grad {

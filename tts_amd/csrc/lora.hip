@@ -188,13 +188,13 @@ constexpr int most(int a, int b) { return a > b ? a : b; }
 constexpr int kPad = 4;                        // floats behind a row of the results' tile: rows start on different banks
 
 // Token rows.  A workgroup takes 16 TT tokens of a segment; its NW waves share the k of the first product (each takes every
-// NW-th 128 bytes of a row: whole lines; 64 bytes were 139 us where these are 133 below, and 16 cache lines a load, not 8) and the output channels of the second, 128 bytes of a
-// row a wave at a time.  The results cross LDS once more, so that base and y are read and written in whole lines.
+// NW-th 128 bytes of a row: whole lines, 8 a load and not 16; 65536 tokens 2048 -> 768 bf16 rank 64 with TT = 2 133 us, with 64 bytes
+// 139) and the output channels of the second, 128 bytes of a row a wave at a time.  The results cross LDS once more, so that base and y are read and written in whole lines.
 // blockIdx.y splits the output channels where there are few tokens; each part then computes h for itself, from cache.
 // EVEN: cin, cout and rank are multiples of a lane's 16 bytes, no place lies in part behind a row.
 // A step's registers are loaded again as soon as LDS has its operands; a second step in flight fits only one rank tile (with
 // two it spilled: 65536 tokens 768 -> 768 bf16 rank 32 81 us, without 64).
-// 65536 tokens 2048 -> 768 bf16 rank 64 with TT = 4: 127 us of 473 MB, 3.7 TB/s (a large copy: 4.7).
+// The call above with TT = 4: 127 us of 473 MB, 3.7 TB/s (a large copy: 4.7).
 // (waves_per_eu: without it accumulators are copied through the second register file and a wave less fits a SIMD.)
 // ACROSS: a is [adapters][cin][rank] and b [adapters][rank][cout], read element by element (the backward pass of one rank tile).
 template <class T, int NW, int RT, int TT, bool EVEN, bool ACROSS = false>
@@ -603,7 +603,7 @@ __device__ __forceinline__ void split3(const float (&v)[8], raw4& hi, raw4& mid,
 // More than 32 ranks are shares of neighbouring workgroups (their sums would leave one wave a SIMD): the channels come from the
 // shared cache again, 65536 tokens 768 / 2048 rank 64 130 us, with the shares one after the other 173.
 // Two steps in flight where the registers of two waves a SIMD hold them (D): the backward pass of 65536 tokens 768 / 2048 rank 8
-// bf16 193 -> 178 us, 32768 tokens 768 / 768 f32 110 -> 98.
+// bf16 198 -> 184 us; f32 gains nothing from it (32768 tokens 768 / 768 rank 8 115 us either way).
 template <class T, int RT, bool EVEN>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))) void lora_weight_kernel(RunTable rt, k82_lora_grad p, const float* gs, float* part) {
     constexpr int V = Vec<T>::N, M = 8, S = sizeof(T), D = RT == 1 ? 2 : 1;          // M: 16 x 16 tiles along the channels
@@ -801,8 +801,10 @@ template <class F> hipError_t by_rank(int rank, F&& f) {
 int parts(int tiles, int cout, int wide) { return std::max(1, std::min((cout + wide - 1) / wide, 512 / std::max(1, tiles))); }
 
 // 64 tokens a workgroup instead of 32, once that leaves two workgroups a CU: the factors are read half as often, which counts
-// where there are more ranks than tokens of a tile.  65536 tokens 768 -> 768 bf16 rank 64 71 us (32 tokens: 84), rank 128 143
-// (174), f32 rank 64 170 (187); with one rank tile 16411 tokens 768 -> 2048 52 (45), 16384 tokens rank 64 32 (21).
+// where there are more ranks than tokens of a tile.  65536 tokens 768 -> 768 bf16 rank 64 72 us (32 tokens: 87), rank 128 143
+// (174), f32 rank 64 173 (194); with one rank tile 65536 tokens 768 -> 2048 243 (154), 16384 tokens rank 64 24 (20).
+// The 32-bit offsets of such a tile reach its 64th row because at least 2^15 rows of that length lie in the card's memory:
+// less than 2^24 bytes each.  (Of 32 rows they reach at the ld of 2^25 that the checks allow.)
 template <class T, int RT> constexpr bool kLargeTiles = RT >= 4;
 template <class T> hipError_t forward(const k82_lora& p, const std::vector<op::Seg>& segs, hipStream_t st, bool across = false) {
     return by_rank(p.rank, [&](auto rt) -> hipError_t {
@@ -849,16 +851,16 @@ int weight_groups(const k82_lora_grad& p) {
     return ((p.cin + 127) / 128 + (p.cout + 127) / 128 + per - 1) / per * ((shares + pair - 1) / pair);
 }
 // Tokens of a chunk of it: as many workgroups a CU as its registers let run at once, two (f32 of more than 16 ranks: three),
-// once there are tokens for them; more would wait for them, and their partial sums are traffic.  The whole backward pass of
-// 65536 tokens 768 / 2048 bf16 rank 16: 512 workgroups 188 us, 768 196; 32768 tokens 768 / 768 bf16 rank 64 79 and 100; 65536
-// tokens 768 / 2048 f32 rank 32 443 and 396.
+// once there are tokens for them; more would wait for them, and their partial sums are traffic.  The whole backward pass with 512
+// workgroups and with 768: 65536 tokens 768 / 2048 bf16 rank 16 190 and 192 us, f32 rank 32 444 and 397; 32768 tokens 768 / 768
+// bf16 rank 64 94 and 107; 8192 tokens bf16 rank 16 32 and 38.  (Against the rule: 65536 tokens f32 rank 16 394 and 366.)
 int chunk_rows(const k82_lora_grad& p, int64_t tokens) {
     const int64_t chunks = std::max<int64_t>(1, (p.rank <= 16 || p.dtype == K82_BF16 ? 512 : 768) / weight_groups(p));
     return (int)std::max<int64_t>(32, ((tokens + chunks - 1) / chunks + 31) / 32 * 32);
 }
 // One rank tile in f32: the factors are read across instead of being transposed first, a launch less (211 tokens 768 -> 768 rank
-// 7 20 us, transposed 21 to 23; 16384 tokens 73 and 76).  Not in bf16, eight loads for 16 bytes (16384 tokens 61 and 56), nor
-// for more ranks (1024 tokens 768 -> 2048 f32 rank 64 66 and 59).
+// 7 23 us, transposed 28; 16384 tokens rank 16 66 and 67).  Not in bf16, eight loads for 16 bytes (16384 tokens 49 and 46), nor
+// for more ranks (1024 tokens 768 -> 2048 f32 rank 64 107 and 82).
 bool reads_across(const k82_lora_grad& p) { return p.dtype == K82_F32 && p.rank <= 16; }
 struct Layout { int64_t g, at, bt, scale, part, end; };         // bytes
 Layout layout(const k82_lora_grad& p, const k82_segments& s) {

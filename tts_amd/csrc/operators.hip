@@ -56,7 +56,7 @@ std::string check_tensor(const char* name, const void* p, int64_t ld, int layout
     if (!p) return optional || tokens == 0 ? "" : std::string(name) + " must not be NULL";
     if ((uintptr_t)p % size) return std::string(name) + " is not aligned to its element";
     if (ld < (layout == K82_COLS ? tokens : c)) return std::string("ld of ") + name + " is smaller than a row of it";
-    if (ld > 1 << 25) return std::string("ld of ") + name + " is larger than 2^25";       // (offsets inside a tile of 32 rows are 32 bits wide)
+    if (ld > 1 << 25) return std::string("ld of ") + name + " is larger than 2^25";       // (offsets inside a tile of rows are 32 bits wide)
     return "";
 }
 std::string check_aligned(int size, std::initializer_list<const void*> p) {
