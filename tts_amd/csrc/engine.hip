@@ -1427,7 +1427,7 @@ struct k82_handle : K82Weights {
 // ============================================================================== C-ABI
 namespace {
 template <class F> int guarded(k82_handle* h, void* stream, F&& f) {
-    if (!h) return K82_EINVAL;
+    if (!h) { g_create_error = "the handle is NULL (or closed)"; return K82_EINVAL; }
     std::lock_guard<std::mutex> lk(h->mu);
     try {
         HIPCHK(hipSetDevice(h->device));
